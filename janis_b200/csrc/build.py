@@ -1,11 +1,12 @@
 """Compiling the CUDA sources for sm_100a and loading them.
 
-There are three kinds of library: `core` (norms, embedding, rotary encoding and
+There are four kinds of library: `core` (norms, embedding, rotary encoding and
 cache write, the 32-bit product, the skinny bfloat16 product, sampling), one
 `attention` library per head size, compiled with that size as a constant, and
 `mixers` (attention whose heads are mixed before the softmax, with values of a
 size of their own; gated linear attention; the state-space scans with their
-convolution; the gated linear recurrence; the gated delta rule; Dynamic Tanh, branch and expert-routing kernels), whose sizes are run-time numbers.  A
+convolution; the gated linear recurrence; the gated delta rule; Dynamic Tanh, branch and expert-routing kernels), whose sizes are run-time numbers, and
+`low_bits` (8-bit rows, 4-bit weights and their products).  A
 library is compiled the first time it is asked for, so a process compiles what
 its model needs and nothing else; the file name carries a hash of the sources
 and flags, so a stale library is never loaded.  The kernels are plain C entry
@@ -37,7 +38,8 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompil
 CORE_SOURCES = ["elementwise.cu", "gemm_f32.cu", "gemv_bf16.cu", "gemm_tc05.cu", "sampling.cu"]
 ATTENTION_SOURCES = ["attention.cu", "attention_prefill_mma.cu", "attention_prefill_tc05.cu", "attention_no_alloc.cu"]
 MIXER_SOURCES = ["attention_talk.cu", "attention_rows.cu", "attention_prep.cu", "linear_attention.cu", "gla_chunks.cu", "delta_rule.cu", "state_space.cu", "duality_scan.cu", "gated_recurrence.cu", "branch_ops.cu", "hyper_streams.cu"]
-HEADERS = ["common.cuh", "attention_no_alloc.h", "attention_prefill_tiles.cuh", "mma_bf16.cuh", "tcgen05.cuh"]
+LOW_BITS_SOURCES = ["mx_rows.cu", "mx_product.cu"]
+HEADERS = ["common.cuh", "attention_no_alloc.h", "attention_prefill_tiles.cuh", "mma_bf16.cuh", "mx.cuh", "tcgen05.cuh"]
 
 
 class BuildError(RuntimeError):
@@ -189,10 +191,15 @@ def mixers_library() -> ctypes.CDLL:
     return _load("janis_mixers", MIXER_SOURCES)
 
 
+def low_bits_library() -> ctypes.CDLL:
+    return _load("janis_low_bits", LOW_BITS_SOURCES)
+
+
 def build_all(head_dims=(16, 32, 64, 128, 256), verbose_ptxas: bool = False) -> list[str]:
-    """Compile the core library and the attention library of each given head size."""
+    """Compile the libraries of one kind each and the attention library of each given head size."""
     paths = [compile_library("janis_core", CORE_SOURCES, verbose_ptxas=verbose_ptxas),
-             compile_library("janis_mixers", MIXER_SOURCES, verbose_ptxas=verbose_ptxas)]
+             compile_library("janis_mixers", MIXER_SOURCES, verbose_ptxas=verbose_ptxas),
+             compile_library("janis_low_bits", LOW_BITS_SOURCES, verbose_ptxas=verbose_ptxas)]
     for hd in head_dims:
         paths.append(compile_library(f"janis_attn_hd{hd}", ATTENTION_SOURCES, [f"JANIS_HEAD_DIM={hd}"],
                                      verbose_ptxas=verbose_ptxas))

@@ -1,0 +1,157 @@
+"""8-bit rows and 4-bit weights: the two microscaling forms, and the kernels that make and take them.
+
+32 values that lie together along a row share a scale that is a power of two.  Rows of activations (`MxRows`) hold e4m3 values,
+weights (`MxWeight`) e2m1 values.  A group's scale is the smallest power of two that brings its largest magnitude under the
+type's largest value (448 and 6), so nothing saturates; a group of zeros has scale 1, a group that holds an infinity or a NaN stands
+for NaN.  `codes` is uint8: [rows, K'] for e4m3 and [N, K' / 2] for e2m1 (the lower half of a byte first), K' the width
+padded to a multiple of 128 with zeros.  `scales` is uint8 [rows / 128, K' / 128, 512] (rounded up): s stands for 2^(s - 127), 255
+for NaN; a block of 512 is [row % 32][row / 32][group], as the tensor cores take it.
+
+The names here are also those of `ops`, whose `rmsnorm`, `add_rmsnorm` and `gated_act` take `MxRows` as their `out`.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops as _ops
+
+GROUP, BLOCK = 32, 128
+
+
+def _padded(k: int) -> int:
+    return (k + BLOCK - 1) // BLOCK * BLOCK
+
+
+class _Mx:
+    """`rows` x `width` values in one of the two forms."""
+
+    __slots__ = ("codes", "scales", "rows", "width")
+    bits = 0
+
+    def __init__(self, codes, scales, rows: int, width: int):
+        rows, width = int(rows), int(width)
+        if rows < 0 or width < 1:
+            raise _ops.KernelError(f"{type(self).__name__}: {rows} rows of {width} values")
+        kp = _padded(width)
+        _ops._t(codes, "codes", torch.uint8, (rows, kp * self.bits // 8))
+        _ops._t(scales, "scales", torch.uint8, (_padded(rows) // BLOCK, kp // BLOCK, 512))
+        if (codes.data_ptr() | scales.data_ptr()) % 32:
+            raise _ops.KernelError(f"{type(self).__name__}: codes and scales must start on 32 bytes")
+        self.codes, self.scales, self.rows, self.width = codes, scales, rows, width
+
+    @classmethod
+    def empty(cls, rows: int, width: int, device="cuda"):
+        """Room for `rows` x `width` values, all zero."""
+        kp = _padded(width)
+        return cls(torch.zeros(rows, kp * cls.bits // 8, dtype=torch.uint8, device=device),
+                   torch.full((_padded(rows) // BLOCK, kp // BLOCK, 512), 127, dtype=torch.uint8, device=device), rows, width)
+
+    @property
+    def shape(self):
+        return (self.rows, self.width)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def values(self, out=None):
+        """The values it stands for, [rows, width] (float32 where no `out` is given)."""
+        if out is None:
+            out = torch.empty(self.rows, self.width, dtype=torch.float32, device=self.codes.device)
+        lib = _ops.low_bits()
+        _ops._check(lib, lib.janis_mx_values(self.codes.data_ptr(), self.scales.data_ptr(), self.bits,
+                                             _ops._t(out, "out", _ops._FLOATS, self.shape), _ops._DT[out.dtype], self.rows, self.width,
+                                             _ops._stream()))
+        return out
+
+
+class MxRows(_Mx):
+    """Rows of activations in 8 bits."""
+    __slots__ = ()
+    bits = 8
+
+
+class MxWeight(_Mx):
+    """Rows of a weight matrix in 4 bits."""
+    __slots__ = ()
+    bits = 4
+
+
+def _rows(x, name, shape):
+    if not isinstance(x, MxRows):
+        raise _ops.KernelError(f"{name}: expected MxRows, found {type(x).__name__}")
+    if x.shape != tuple(shape):
+        raise _ops.KernelError(f"{name}: shape {x.shape} does not match {tuple(shape)}")
+    return x.codes.data_ptr(), x.scales.data_ptr()
+
+
+def mx_rows(x, out: MxRows) -> MxRows:
+    """out = x [R, K] in 8 bits."""
+    R, K = x.shape
+    lib = _ops.low_bits()
+    _ops._check(lib, lib.janis_mx_rows(_ops._t(x, "x", _ops._FLOATS), _ops._DT[x.dtype], -1, 0.0, 0.0, 0.0, *_rows(out, "out", (R, K)), R, K,
+                                       _ops._stream()))
+    return out
+
+
+def mx_weight(w) -> MxWeight:
+    """A weight matrix w [N, K] in 4 bits."""
+    N, K = w.shape
+    p, out, lib = _ops._t(w, "w", _ops._FLOATS), MxWeight.empty(N, K, w.device), _ops.low_bits()
+    _ops._check(lib, lib.janis_mx_weight(p, _ops._DT[w.dtype], out.codes.data_ptr(), out.scales.data_ptr(), N, K, _ops._stream()))
+    return out
+
+
+def norm_to_rows(h, res, w_post, eps_post, w_next, eps_next, out: MxRows, n_part: int = 1, rows=None) -> MxRows:
+    """`rmsnorm` (res None) and `add_rmsnorm` with 8-bit rows as their output."""
+    H = h.shape[1]
+    R = out.rows if res is None else h.shape[0]
+    if w_next is None:
+        raise _ops.KernelError("add_rmsnorm: 8-bit rows are the second norm's output, which has no weight here")
+    if res is None:
+        if rows is None and h.shape[0] != R:
+            raise _ops.KernelError(f"rmsnorm: {h.shape[0]} input rows for {R} output rows")
+        p_res, dt, stride = None, 0, 0
+    else:
+        p_res, dt, stride = _ops._t(res, "res", _ops._FLOATS, (R, H) if n_part == 1 else (n_part, R, H)), _ops._DT[res.dtype], R * H
+    lib = _ops.low_bits()
+    _ops._check(lib, lib.janis_mx_norm_rows(
+        _ops._t(h, "h", torch.float32, (None, H)), p_res, dt, n_part, stride,
+        _ops._t(w_post, "w_post", torch.float32, (H,)) if w_post is not None else None, float(eps_post),
+        _ops._t(w_next, "w_next", torch.float32, (H,)), float(eps_next), _ops._t(rows, "rows", torch.int32, (R,)) if rows is not None else None,
+        *_rows(out, "out", (R, H)), R, H, _ops._stream()))
+    return out
+
+
+def gated_to_rows(gu, out: MxRows, act: int, group: int, limit: float, alpha: float, up_add: float) -> MxRows:
+    """`gated_act` with 8-bit rows as its output."""
+    R, I2 = gu.shape
+    if group != _ops.GATE_GROUP:
+        raise _ops.KernelError(f"gated_act: 8-bit rows come from gates and ups in groups of {_ops.GATE_GROUP}, found {group}")
+    lib = _ops.low_bits()
+    _ops._check(lib, lib.janis_mx_rows(_ops._t(gu, "gu", _ops._FLOATS), _ops._DT[gu.dtype], int(act), float(limit), float(alpha), float(up_add),
+                                       *_rows(out, "out", (R, I2 // 2)), R, I2 // 2, _ops._stream()))
+    return out
+
+
+def linear_mx(x: MxRows, w: MxWeight, out, epilogue: int = 0, limit: float = 0.0, alpha: float = 1.0, up_add: float = 0.0):
+    """out[T, N] = x w^T of 8-bit rows and 4-bit weights, float sums; out bfloat16 or float32.  With a gated epilogue
+    (EPI_GATED_GELU, EPI_GATED_SILU, EPI_GATED_CLAMP with its three numbers) the rows of w alternate 8 gates, 8 ups and
+    out[T, N / 2] = act(gate) * up; it may be `MxRows` then."""
+    if not isinstance(w, MxWeight):
+        raise _ops.KernelError(f"linear_mx: w must be MxWeight, found {type(w).__name__}")
+    T, K, N = x.rows, x.width, w.rows
+    if w.width != K:
+        raise _ops.KernelError(f"linear_mx: x has {K} columns and w {w.width}")
+    gated = epilogue != _ops.EPI_NONE
+    shape = (T, N // 2 if gated else N)
+    if isinstance(out, MxRows):
+        if not gated:
+            raise _ops.KernelError("linear_mx: 8-bit rows are a gated epilogue's output")
+        p_out, dt, (pc, ps) = None, 0, _rows(out, "out", shape)
+    else:
+        p_out, dt, pc, ps = _ops._t(out, "out", _ops._FLOATS, shape), _ops._DT[out.dtype], None, None
+    lib = _ops.low_bits()
+    _ops._check(lib, lib.janis_mx_product(*_rows(x, "x", (T, K)), w.codes.data_ptr(), w.scales.data_ptr(), p_out, dt, pc, ps, T, N, K,
+                                          int(epilogue), float(limit), float(alpha), float(up_add), _ops._stream()))
+    return out

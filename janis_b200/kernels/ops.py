@@ -201,6 +201,28 @@ def mixers():
     return _mixers
 
 
+_low_bits = None
+
+
+def low_bits():
+    """The library of 8-bit rows and 4-bit weights (compiled when a model first needs it)."""
+    global _low_bits
+    if _low_bits is None:
+        _need_cuda()
+        lib = build.low_bits_library()
+        P, I, F = c_void_p, c_int, c_float
+        lib.janis_mx_norm_rows.argtypes = [P, P, I, I, c_longlong, P, F, P, F, P, P, P, I, I, P]
+        lib.janis_mx_rows.argtypes = [P, I, I, F, F, F, P, P, I, I, P]
+        lib.janis_mx_weight.argtypes = [P, I, P, P, I, I, P]
+        lib.janis_mx_values.argtypes = [P, P, I, P, I, I, I, P]
+        lib.janis_mx_product.argtypes = [P, P, P, P, P, I, P, P, I, I, I, I, F, F, F, P]
+        lib.janis_mx_set_overlap.argtypes = [I]
+        lib.janis_mx_set_overlap.restype = None
+        lib.janis_mx_set_overlap(1 if _overlap else 0)
+        _low_bits = lib
+    return _low_bits
+
+
 _overlap = os.environ.get("JANIS_OVERLAP", "1") != "0"
 
 
@@ -216,6 +238,8 @@ def set_overlap(on: bool) -> None:
         lib.janis_attn_set_overlap(1 if _overlap else 0)
     if _mixers is not None:
         _mixers.janis_mixers_set_overlap(1 if _overlap else 0)
+    if _low_bits is not None:
+        _low_bits.janis_mx_set_overlap(1 if _overlap else 0)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -295,7 +319,10 @@ def embed(tokens, table, scale: float, out):
 
 
 def rmsnorm(x, weight, eps: float, out, rows=None):
-    """out[r] = x[rows[r] or r] / sqrt(mean(x^2) + eps) * weight;  weight float32 holds offset + w."""
+    """out[r] = x[rows[r] or r] / sqrt(mean(x^2) + eps) * weight;  weight float32 holds offset + w.  `out` may be `MxRows`
+    (of float32 x)."""
+    if type(out) is MxRows:
+        return mx.norm_to_rows(x, None, None, 0.0, weight, eps, out, rows=rows)
     H = x.shape[-1]
     R = out.shape[0]
     if rows is None and x.shape[0] != R:
@@ -310,7 +337,9 @@ def rmsnorm(x, weight, eps: float, out, rows=None):
 def add_rmsnorm(h, res, w_post, eps_post, w_next=None, eps_next=0.0, out=None, n_part=1):
     """h += norm(res; w_post) in place (float32 residual sum; h += res when w_post is None);
     out = norm(h; w_next) when w_next is given.
-    `res` is [R, H], or [n_part, R, H] partial results that are added first."""
+    `res` is [R, H], or [n_part, R, H] partial results that are added first.  `out` may be `MxRows`."""
+    if type(out) is MxRows:
+        return mx.norm_to_rows(h, res, w_post, eps_post, w_next, eps_next, out, n_part)
     R, H = h.shape
     if n_part == 1:
         _t(res, "res", _FLOATS, (R, H))
@@ -332,7 +361,9 @@ def gated_act(gu, out, act: int = ACT_GELU_TANH, group: int = GATE_GROUP, limit:
               up_add: float = 0.0):
     """out[r, j] = act(gate) * up over a fused [R, 2I] product whose columns alternate
     `group` gate columns and `group` up columns.  ACT_CLAMPED takes three numbers: g sigmoid(alpha g) (u + up_add) with
-    g = min(gate, limit), u = clamp(up, -limit, limit)."""
+    g = min(gate, limit), u = clamp(up, -limit, limit).  `out` may be `MxRows`."""
+    if type(out) is MxRows:
+        return mx.gated_to_rows(gu, out, act, group, limit, alpha, up_add)
     R, I2 = gu.shape
     I = I2 // 2
     lib = core()
@@ -1878,3 +1909,7 @@ def mask_tokens(logits, ids):
     _check(lib, lib.janis_mask_tokens(_t(logits, "logits", torch.float32), _t(ids, "ids", torch.int32), ids.numel(),
                                       R, V, _stream()))
     return logits
+
+
+from . import mx                                                          # noqa: E402  (it uses the helpers above)
+from .mx import MxRows, MxWeight, linear_mx, mx_rows, mx_weight           # noqa: E402
