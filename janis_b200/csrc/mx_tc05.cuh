@@ -1,0 +1,76 @@
+// What the products of the microscaling forms use of the 5th-generation tensor cores: block-scaled products of e4m3 with e2m1,
+// scales brought from shared to tensor memory, plain bulk copies, tensor maps of both forms.
+//
+// e2m1 values come packed through the copy engine, which spreads them: 16 of them fill the lower 8 of 16 bytes in shared memory, so
+// that a row of 128 values takes 128 bytes there like a row of e4m3, under the same 128-byte swizzle.  An mbarrier counts the
+// packed bytes.
+#pragma once
+
+#include <mutex>
+
+#include "mx.cuh"
+#include "tcgen05.cuh"
+
+namespace janis {
+namespace mx {
+
+enum Side { WEIGHTS, ROWS };       // e2m1 and e4m3
+
+// kind::mxf8f6f4, both operands K-major, shape M x N x 32, float sums; `group`: which of the four scales of a lane the products take
+template <Side A>
+__device__ __forceinline__ uint32_t block_desc(int M, int N, int group) {
+    constexpr uint32_t a = A == WEIGHTS ? 5u : 0u, b = A == WEIGHTS ? 0u : 5u;       // 5: e2m1, 0: e4m3
+    return ((uint32_t)group << 4) | (a << 7) | (b << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27) |
+           ((uint32_t)group << 29);
+}
+__device__ __forceinline__ void umma_block(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %6, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+}
+// a block of scales (32 lanes x 16 bytes, contiguous) into four columns of all four quarters of tensor memory; in order before
+// the products that the same thread issues after it
+__device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t smem) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem & 0x3FFFF) >> 4);
+    d |= (uint64_t)1 << 16;
+    d |= (uint64_t)(128 >> 4) << 32;                    // groups of 8 lanes 128 bytes apart, no swizzle
+    d |= (uint64_t)1 << 46;
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(d) : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes),
+                 "r"(bar)
+                 : "memory");
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiled encoder() {
+    static EncodeTiled fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiled)p;
+    });
+    return fn;
+}
+// [rows, kp] values, kp a multiple of 128, in boxes of 128 x box_rows; rows past the end are zeros
+inline bool make_map(CUtensorMap* map, Side side, const void* codes, int rows, int kp, int box_rows) {
+    EncodeTiled enc = encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)kp, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(side == WEIGHTS ? kp / 2 : kp)};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+    const cuuint32_t elem[2] = {1, 1};
+    return enc(map, side == WEIGHTS ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims,
+               strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace mx
+}  // namespace janis

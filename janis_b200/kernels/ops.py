@@ -216,6 +216,9 @@ def low_bits():
         lib.janis_mx_weight.argtypes = [P, I, P, P, I, I, P]
         lib.janis_mx_values.argtypes = [P, P, I, P, I, I, I, P]
         lib.janis_mx_product.argtypes = [P, P, P, P, P, I, P, P, I, I, I, I, F, F, F, P]
+        lib.janis_mx_set_few.argtypes = [I, I]
+        lib.janis_mx_set_few.restype = None
+        lib.janis_mx_timeouts_async.argtypes = [P, P]
         lib.janis_mx_set_overlap.argtypes = [I]
         lib.janis_mx_set_overlap.restype = None
         lib.janis_mx_set_overlap(1 if _overlap else 0)
@@ -607,6 +610,8 @@ class WaitWatch:
         st, base = _stream(), self._host.data_ptr()
         if _core is not None:
             _check(_core, _core.janis_tc05_timeouts_async(base + 4 * self._slot("core"), st), 0)
+        if _low_bits is not None:
+            _check(_low_bits, _low_bits.janis_mx_timeouts_async(base + 4 * self._slot("low_bits"), st), 0)
         for hd, lib in _attn.items():
             _check(lib, lib.janis_attn_timeouts_async(base + 4 * self._slot(f"attention (head size {hd})"), st), 0)
 
