@@ -20,7 +20,7 @@ import sys
 import time
 
 USAGE = """usage: janis generate --model DIR (--ids 1,2,3 | --ids-file FILE) [--temp 0] [--top-p 1] [--max-tokens 512]
-                      [--seed 0] [--stop 1,107] [--dtype bfloat16|float32] [--max-cache-tokens N]
+                      [--seed 0] [--stop 1,107] [--dtype bfloat16|float32] [--max-cache-tokens N] [--weights mx4]
        janis generate --random CONFIG.json [--weights-seed 0] ...   (random weights instead of a folder)
        janis replay   --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N   < steps.jsonl
        janis random   --config CONFIG.json --out DIR [--seed 0]     (write a folder of random weights)
@@ -61,6 +61,7 @@ def cmd_generate(argv) -> int:
     ap.add_argument("--stop", default=None, help="stop token ids (default: the model's end-of-sequence ids)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
     ap.add_argument("--max-cache-tokens", type=int, default=0)
+    ap.add_argument("--weights", default=None, choices=["mx4"], help="keep the layers' matrices in 4 bits")
     a = ap.parse_args(argv)
     prompts = [_ids(s) for s in a.ids]
     if a.ids_file:
@@ -73,10 +74,11 @@ def cmd_generate(argv) -> int:
     need = sum((len(p) + a.max_tokens + 63) // 64 * 64 for p in prompts)
     cache_tokens = a.max_cache_tokens or min(need, 1 << 20)
     if a.model:
-        eng = janis_b200.open(a.model, dtype=a.dtype, max_tokens=cache_tokens)
+        eng = janis_b200.open(a.model, dtype=a.dtype, max_tokens=cache_tokens, weights=a.weights)
     else:
         with open(a.random) as f:
-            eng = janis_b200.from_config(json.load(f), seed=a.weights_seed, dtype=a.dtype, max_tokens=cache_tokens)
+            eng = janis_b200.from_config(json.load(f), seed=a.weights_seed, dtype=a.dtype, max_tokens=cache_tokens,
+                                         weights=a.weights)
     t0 = time.time()
     replies = eng.generate(prompts, temp=a.temp, top_p=a.top_p, max_tokens=a.max_tokens, seed=a.seed,
                            stop=_ids(a.stop) if a.stop is not None else None,

@@ -202,11 +202,19 @@ class _Backend:
 # opening
 # ---------------------------------------------------------------------------
 
-def _runtime(dtype, device) -> Runtime:
+def _runtime(dtype, device, weights=None) -> Runtime:
     if not torch.cuda.is_available():
         raise RuntimeError("janis_b200 needs a CUDA device (sm_100a); none is visible and there is no "
                            "CPU implementation")
-    return Runtime(_dtype(dtype), device, cuda_ops)
+    return Runtime(_dtype(dtype), device, cuda_ops, weights)
+
+
+def check_low_bits(model) -> None:
+    """Refuses a model some of whose layers cannot keep their matrices in 4 bits."""
+    for i, blk in enumerate(model.blocks):
+        for part in (blk, blk.mixer, getattr(blk, "feed_forward", None)):
+            if part is not None and not part.low_bits:
+                raise ValueError(f"weights='mx4': {type(part).__name__} (layer {i}) takes its matrices in the compute dtype only")
 
 
 def build_model(raw_config: dict, where: str = "config.json"):
@@ -218,15 +226,19 @@ def build_model(raw_config: dict, where: str = "config.json"):
 
 def open(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, max_batch: int | None = None,
          max_context: int | None = None, device="cuda:0", use_graphs: bool = True,
-         max_step_tokens: int = 16384) -> Engine:
+         max_step_tokens: int = 16384, weights: str | None = None) -> Engine:
     """Load config.json and the safetensors of `model_dir` and build the engine.
 
     `max_tokens` is how many tokens the cache holds over all live sequences (each
     sequence's count rounded up to whole pages of 64); `max_batch` bounds the sequences
-    alive at once (default: as many as there are pages)."""
+    alive at once (default: as many as there are pages).  `weights="mx4"` keeps the layers' matrices in 4 bits with a
+    scale for every 32 values (converted as they are loaded) and gives their products 8-bit rows; the embedding and the
+    output head stay in `dtype`."""
     raw = read_config_json(model_dir)
     _, cfg, model = build_model(raw, os.path.join(model_dir, "config.json"))
-    rt = _runtime(dtype, device)
+    rt = _runtime(dtype, device, weights)
+    if rt.weights:
+        check_low_bits(model)
     store = WeightStore(load_tensors(model_dir, model.tensor_specs(), rt.device, model.ignorable_tensors))
     model.load(store, rt)         # parts that fuse tensors give the stored ones up as they go
     del store
@@ -238,10 +250,12 @@ load = open     # the same call under the name that Python libraries usually giv
 
 def from_config(raw_config: dict, seed: int = 0, dtype="bfloat16", max_tokens: int = 8192,
                 max_batch: int | None = None, max_context: int | None = None, device="cuda:0",
-                use_graphs: bool = True, max_step_tokens: int = 16384) -> Engine:
+                use_graphs: bool = True, max_step_tokens: int = 16384, weights: str | None = None) -> Engine:
     """An engine with random weights drawn on the device from (seed, tensor name): no folder is written."""
     _, cfg, model = build_model(raw_config, "config")
-    rt = _runtime(dtype, device)
+    rt = _runtime(dtype, device, weights)
+    if rt.weights:
+        check_low_bits(model)
     store = WeightStore(random_tensors(model.tensor_specs(), seed, rt.device))
     model.load(store, rt)
     del store

@@ -76,6 +76,13 @@ class MxWeight(_Mx):
     __slots__ = ()
     bits = 4
 
+    def __getitem__(self, rows: slice) -> "MxWeight":
+        """Its first rows, over the same memory."""
+        if not isinstance(rows, slice) or rows.start not in (None, 0) or rows.step not in (None, 1):
+            raise IndexError("4-bit weights are cut behind their first rows only: w[:n]")
+        n = len(range(*rows.indices(self.rows)))
+        return MxWeight(self.codes[:n], self.scales[:_padded(n) // BLOCK], n, self.width)
+
 
 def _rows(x, name, shape):
     if not isinstance(x, MxRows):
@@ -134,12 +141,17 @@ def gated_to_rows(gu, out: MxRows, act: int, group: int, limit: float, alpha: fl
     return out
 
 
+def mx_set_few(split: int = 0, stages: int = 0) -> None:
+    """Fixes how many CTAs share K (1, 2, 4, 8) and the depth of the ring in products of few rows (0: chosen).  For tests and tuning."""
+    _ops.low_bits().janis_mx_set_few(int(split), int(stages))
+
+
 def linear_mx(x: MxRows, w: MxWeight, out, epilogue: int = 0, limit: float = 0.0, alpha: float = 1.0, up_add: float = 0.0):
     """out[T, N] = x w^T of 8-bit rows and 4-bit weights, float sums; out bfloat16 or float32.  With a gated epilogue
     (EPI_GATED_GELU, EPI_GATED_SILU, EPI_GATED_CLAMP with its three numbers) the rows of w alternate 8 gates, 8 ups and
     out[T, N / 2] = act(gate) * up; it may be `MxRows` then."""
-    if not isinstance(w, MxWeight):
-        raise _ops.KernelError(f"linear_mx: w must be MxWeight, found {type(w).__name__}")
+    if type(x) is not MxRows or type(w) is not MxWeight:
+        raise _ops.KernelError(f"linear_mx: x must be MxRows and w MxWeight, found {type(x).__name__} and {type(w).__name__}")
     T, K, N = x.rows, x.width, w.rows
     if w.width != K:
         raise _ops.KernelError(f"linear_mx: x has {K} columns and w {w.width}")

@@ -1917,4 +1917,4 @@ def mask_tokens(logits, ids):
 
 
 from . import mx                                                          # noqa: E402  (it uses the helpers above)
-from .mx import MxRows, MxWeight, linear_mx, mx_rows, mx_weight           # noqa: E402
+from .mx import MxRows, MxWeight, linear_mx, mx_rows, mx_set_few, mx_weight           # noqa: E402

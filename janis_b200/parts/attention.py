@@ -86,6 +86,8 @@ def gathered_room(ctx: StepContext, n_kv_heads: int, head_dim: int) -> dict:
 
 
 class SoftmaxAttention(Mixer):
+    low_bits = True
+
     def __init__(self, hidden: int, n_heads: int, n_kv_heads: int, head_dim: int, scale: float,
                  position: PositionEncoding, names: dict[str, str], softcap: float = 0.0,
                  window: int | None = None, init_std: float = 0.02):
@@ -131,12 +133,14 @@ class SoftmaxAttention(Mixer):
         if rt.dtype == torch.bfloat16 and (self.hidden % 8 or (self.n_heads * self.head_dim) % 8):
             raise ValueError("the bfloat16 products need widths that are multiples of 8 "
                              f"(hidden {self.hidden}, heads x head size {self.n_heads * self.head_dim})")
-        q, k, v = (store.get(self.names[n], rt.dtype) for n in ("q", "k", "v"))
-        self.w_qkv = torch.cat([q, k, v], dim=0).contiguous()
+        q, k, v = (store.get(self.names[n], rt.weight_dtype) for n in ("q", "k", "v"))
+        self.w_qkv = rt.weight(torch.cat([q, k, v], dim=0))
         del q, k, v
         store.drop(self.names["q"], self.names["k"], self.names["v"])      # the fused copy is the one that stays
         self.w_q = self.w_qkv[: self.n_heads * self.head_dim]      # a layer that only reads keys projects q alone
-        self.w_o = store.get(self.names["o"], rt.dtype).contiguous()
+        self.w_o = rt.weight(store.get(self.names["o"], rt.weight_dtype))
+        if rt.weights:
+            store.drop(self.names["o"])
         self.position.load(store, rt)
 
     # -- a step ------------------------------------------------------------

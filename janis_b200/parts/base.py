@@ -54,11 +54,17 @@ from ..weights.loader import TensorSpec
 
 class Runtime:
     """The compute dtype, the device and the kernels a model runs with.  `over(ws)`: the same with a workspace, in which
-    the products keep the room they need from step to step; without one they ask the allocator."""
+    the products keep the room they need from step to step; without one they ask the allocator.
 
-    def __init__(self, dtype: torch.dtype, device, ops):
+    weights="mx4": the layers' matrices are kept in 4 bits (`MxWeight`) and their products take 8-bit rows (`MxRows`); the
+    norms and the gated activation in front of them leave such rows.  What is between the products stays in the compute dtype."""
+
+    def __init__(self, dtype: torch.dtype, device, ops, weights: str | None = None):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype must be float32 or bfloat16, found {dtype}")
+        if weights not in (None, "mx4"):
+            raise ValueError(f"weights must be None (the compute dtype) or 'mx4', found {weights!r}")
+        self.weights = weights
         self.dtype = dtype
         self.device = device
         self.ops = ops
@@ -67,8 +73,30 @@ class Runtime:
         self.sm_count = (torch.cuda.get_device_properties(dev).multi_processor_count
                          if dev.type == "cuda" else 1)
 
-    def linear(self, x: torch.Tensor, w: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-        """out = x w^T in the compute dtype, accumulated in float32."""
+    @property
+    def weight_dtype(self):
+        """The type in which a layer takes its matrices from the store: for 4 bits as they are stored (None), since rounding to
+        bfloat16 first would turn one code in a hundred or so by a quarter to a half of its value."""
+        return None if self.weights == "mx4" else self.dtype
+
+    def weight(self, w: torch.Tensor):
+        """A matrix of a layer's product as the product takes it: as it is, or in 4 bits."""
+        return self.ops.mx_weight(w.contiguous()) if self.weights == "mx4" else w.contiguous()
+
+    def rows(self, ws: "Workspace", name: str, n_rows: int, width: int):
+        """Room for the rows a layer's product reads: in the compute dtype, or in 8 bits."""
+        if self.weights == "mx4":
+            return ws.mx_rows(name, n_rows, width, self.ops.MxRows)
+        return ws.buf(name, (n_rows, width), self.dtype)
+
+    def linear(self, x, w, out: torch.Tensor) -> torch.Tensor:
+        """out = x w^T in the compute dtype, accumulated in float32.  A w in 4 bits takes x in 8 bits, or brings it there."""
+        if not isinstance(w, torch.Tensor):
+            if isinstance(x, torch.Tensor):
+                if self.ws is None:
+                    raise ValueError("a product with 4-bit weights needs a workspace for its 8-bit rows")
+                x = self.ops.mx_rows(x, self.ws.mx_rows("linear.x", *x.shape, self.ops.MxRows))
+            return self.ops.linear_mx(x, w, out)
         if self.dtype == torch.float32:
             return self.product_f32(x, w, out)
         return self.ops.linear_bf16(x, w, out)
@@ -98,6 +126,7 @@ class Workspace:
         self._in_graph: set[str] = set()          # names whose current buffer a CUDA graph has recorded
         self._retired: list[torch.Tensor] = []    # outgrown buffers that a graph still writes to
         self._views: dict[str, tuple] = {}        # name -> (shape, buffer, view): the view handed out last
+        self._rows: dict = {}                     # name -> the 8-bit rows handed out last
 
     def buf(self, name: str, shape, dtype: torch.dtype) -> torch.Tensor:
         shape = tuple(shape)
@@ -129,6 +158,16 @@ class Workspace:
         view = cur[:n].view(*shape)
         self._views[name] = (shape, cur, view)
         return view
+
+    def mx_rows(self, name: str, n_rows: int, width: int, cls):
+        """The same for rows in 8 bits (`cls`: the kernels' `MxRows`).  Whoever writes such rows writes their padding too."""
+        kp = -(-width // 128) * 128
+        codes = self.buf(name + ".codes", (n_rows, kp), torch.uint8)
+        scales = self.buf(name + ".scales", (-(-n_rows // 128), kp // 128, 512), torch.uint8)
+        last = self._rows.get(name)
+        if last is None or last.codes is not codes or last.scales is not scales or last.width != width:
+            last = self._rows[name] = cls(codes, scales, n_rows, width)
+        return last
 
     def fill(self, value) -> None:
         """Every buffer filled with `value` (tests poison the workspace with NaN between steps: a step must write
@@ -181,6 +220,8 @@ class Part:
     # leaves it True meets padding in recorded steps, decode and prompt steps alike: sequences whose slot is
     # negative (and the tokens that name them) must be stored nowhere and must change no other row.
     graph_safe = True
+    # whether a block, mixer or feed-forward keeps its matrices through `rt.weight` and takes its rows as `rt.rows` gives them
+    low_bits = False
 
     def tensor_specs(self) -> dict[str, TensorSpec]:
         return {}

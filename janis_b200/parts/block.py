@@ -28,6 +28,8 @@ import torch
 
 
 class SandwichBlock(Block):
+    low_bits = True
+
     def __init__(self, mixer: Mixer, feed_forward: FeedForward | None, input_norm: Norm, post_mixer_norm: Norm,
                  pre_ff_norm: Norm | None = None, post_ff_norm: Norm | None = None):
         if feed_forward is not None and (pre_ff_norm is None or post_ff_norm is None):
@@ -44,16 +46,15 @@ class SandwichBlock(Block):
 
     def forward(self, h, ctx: StepContext, line, y_in=None, next_norm: Norm | None = None):
         T, H = h.shape
-        dt = ctx.rt.dtype
-        y = y_in if y_in is not None else self.first_norm.forward(h, ctx, ctx.ws.buf("block.y", (T, H), dt))
+        y = y_in if y_in is not None else self.first_norm.forward(h, ctx, ctx.rt.rows(ctx.ws, "block.y", T, H))
         r = self.mixer.forward(y, ctx, line)
         if self.feed_forward is None:
-            return h, self.post_mixer_norm.residual_add(h, r, ctx, next_norm, ctx.ws.buf("block.y", (T, H), dt)
+            return h, self.post_mixer_norm.residual_add(h, r, ctx, next_norm, ctx.rt.rows(ctx.ws, "block.y", T, H)
                                                         if next_norm is not None else None)
-        y = self.post_mixer_norm.residual_add(h, r, ctx, self.pre_ff_norm, ctx.ws.buf("block.y", (T, H), dt))
+        y = self.post_mixer_norm.residual_add(h, r, ctx, self.pre_ff_norm, ctx.rt.rows(ctx.ws, "block.y", T, H))
         r = self.feed_forward.forward(y, ctx)
         y_next = self.post_ff_norm.residual_add(h, r, ctx, next_norm,
-                                                ctx.ws.buf("block.y", (T, H), dt) if next_norm is not None else None)
+                                                ctx.rt.rows(ctx.ws, "block.y", T, H) if next_norm is not None else None)
         return h, y_next
 
 

@@ -27,6 +27,7 @@ _ACTS = {"gelu_tanh": 0, "gelu_pytorch_tanh": 0, "silu": 1, "clamped_swish": 2}
 
 class GatedMLP(FeedForward):
     GROUP = 8
+    low_bits = True
 
     def __init__(self, hidden: int, intermediate: int, names: dict[str, str], act: str = "gelu_tanh",
                  init_std: float = 0.02, limit: float | None = None, gate_alpha: float = 1.702):
@@ -55,27 +56,31 @@ class GatedMLP(FeedForward):
                 self.names["down"]: TensorSpec((H, I), init_std=s)}
 
     def load(self, store, rt: Runtime):
-        g = store.get(self.names["gate"], rt.dtype)
-        u = store.get(self.names["up"], rt.dtype)
+        g = store.get(self.names["gate"], rt.weight_dtype)
+        u = store.get(self.names["up"], rt.weight_dtype)
         I, H, G = self.padded, self.hidden, self.GROUP
         if I != self.intermediate:
             pad = torch.zeros(I - self.intermediate, H, dtype=g.dtype, device=g.device)
             g, u = torch.cat([g, pad]), torch.cat([u, pad])
         fused = torch.stack([g.view(I // G, G, H), u.view(I // G, G, H)], dim=1)   # [I/G, 2, G, H]
-        self.w_gu = fused.reshape(2 * I, H).contiguous()
+        self.w_gu = rt.weight(fused.reshape(2 * I, H))
         del g, u, fused
         store.drop(self.names["gate"], self.names["up"])                   # the fused copy is the one that stays
-        self.w_down = store.get(self.names["down"], rt.dtype).contiguous()
+        down = store.get(self.names["down"], rt.weight_dtype)
         if I != self.intermediate:
-            self.w_down = torch.cat([self.w_down, torch.zeros(H, I - self.intermediate, dtype=self.w_down.dtype,
-                                                              device=self.w_down.device)], dim=1).contiguous()
+            down = torch.cat([down, torch.zeros(H, I - self.intermediate, dtype=down.dtype, device=down.device)], dim=1)
+        self.w_down = rt.weight(down)
+        if rt.weights:
+            store.drop(self.names["down"])
 
     def forward(self, x, ctx: StepContext):
         rt, ws, ops = ctx.rt, ctx.ws, ctx.rt.ops
         T, I = ctx.n_tok, self.padded
-        a = ws.buf("ffn.act", (T, I), rt.dtype)
+        a = rt.rows(ws, "ffn.act", T, I)
         epi = (ops.EPI_GATED_GELU, ops.EPI_GATED_SILU, ops.EPI_GATED_CLAMP)[self.act]
-        if rt.dtype == torch.bfloat16 and T <= ops.GEMV_FAST_ROWS and self.hidden % 8 == 0:   # (the skinny product reads 16 bytes at a time)
+        if rt.weights:
+            ops.linear_mx(x, self.w_gu, a, epi, **self.extra)
+        elif rt.dtype == torch.bfloat16 and T <= ops.GEMV_FAST_ROWS and self.hidden % 8 == 0:   # (the skinny product reads 16 bytes at a time)
             ops.gemv_bf16(x, self.w_gu, a, epi, **({"cap": self.extra["limit"], "alpha": self.extra["alpha"],
                                                     "up_add": self.extra["up_add"]} if self.extra else {}))
         else:

@@ -117,7 +117,7 @@ class RotaryEncoding(PositionEncoding):
         write are one kernel (the product's tiles pair each element with its partner half a head on)."""
         self._halves_only()
         ops = ctx.rt.ops
-        fused = (ctx.mode == "decode" and ctx.rt.dtype == torch.bfloat16 and self.rot == hd and hd % 16 == 0
+        fused = (isinstance(w, torch.Tensor) and ctx.mode == "decode" and ctx.rt.dtype == torch.bfloat16 and self.rot == hd and hd % 16 == 0
                  and x.shape[0] <= getattr(ops, "GEMV_FAST_ROWS", 0) and hasattr(ops, "gemv_rope_store"))
         if not fused:
             return super().project_encode_store(x, w, qkv, ctx, nq, nkv, hd, kv_line)

@@ -20,6 +20,75 @@ GATE_GROUP = 8
 ACT_GELU_TANH, ACT_SILU, ACT_CLAMPED = 0, 1, 2
 
 
+class MxRows:
+    """8-bit rows, by the formats' definitions (see `tests/test_low_bits.py: quantised`)."""
+    dtype = torch.float64
+    limit, digits, low = 448.0, 3, -6            # the largest value, the mantissa's bits, the exponent of the least normal value
+
+    def __init__(self, codes, scales, rows, width):
+        self.codes, self.scales, self.rows, self.width = codes, scales, rows, width
+        self.held = torch.zeros(rows, width, dtype=torch.float64)
+
+    @property
+    def shape(self):
+        return (self.rows, self.width)
+
+    def copy_(self, v):
+        self.held = quantised(v.double(), self.limit, self.digits, self.low)[0]
+        return self
+
+    def values(self):
+        return self.held
+
+
+class MxWeight(MxRows):
+    limit, digits, low = 6.0, 1, 0
+
+    def __getitem__(self, rows):
+        w = MxWeight(None, None, len(range(*rows.indices(self.rows))), self.width)
+        w.held = self.held[rows]
+        return w
+
+
+def quantised(v, limit, digits, low):
+    """(values, codes' values, scales) of rows in groups of 32 with the smallest power of two that brings each under `limit`;
+    codes have `digits` bits behind the point and exponents from `low` on, ties go to the even one."""
+    r, k = v.shape
+    kp = -(-k // 128) * 128
+    g = torch.zeros(r, kp, dtype=torch.float64, device=v.device)
+    g[:, :k] = v
+    g = g.view(r, kp // 32, 32)
+    big = g.abs().amax(-1, keepdim=True)
+    m, e = torch.frexp(big / limit)
+    e = torch.where(big > 0, torch.where(m == 0.5, e - 1, e).clamp(min=-127), torch.zeros_like(e)).double()
+    scale = torch.where(torch.isfinite(big), torch.ldexp(torch.ones_like(big), e.int()), torch.full_like(big, float("nan")))
+    q = torch.where(torch.isfinite(big), g / scale, torch.zeros_like(g))
+    _, at = torch.frexp(q)
+    step = torch.ldexp(torch.ones_like(q), (at - 1).clamp(min=low) - digits)
+    q = torch.round(q / step) * step
+    return (q * scale).view(r, kp)[:, :k], q.view(r, kp), scale[..., 0]
+
+
+def mx_rows(x, out):
+    return out.copy_(x)
+
+
+def mx_weight(w):
+    return MxWeight(None, None, *w.shape).copy_(w)
+
+
+def linear_mx(x, w, out, epilogue=EPI_NONE, limit=0.0, alpha=1.0, up_add=0.0):
+    v = x.values() @ w.values().T
+    if epilogue != EPI_NONE:
+        t, n = v.shape
+        gate, up = v.view(t, n // 16, 2, 8).unbind(2)
+        gate, up = gate.reshape(t, n // 2), up.reshape(t, n // 2)
+        v = _clamped(gate, up, limit, alpha, up_add) if epilogue == EPI_GATED_CLAMP else \
+            _act(gate, ACT_GELU_TANH if epilogue == EPI_GATED_GELU else ACT_SILU) * up
+    out.copy_(v if isinstance(out, MxRows) else v.to(out.dtype))
+    return out
+
+
 def embed(tokens, table, scale, out):
     out.copy_((table[tokens.long()].double() * float(np.float32(scale))).to(out.dtype))
     return out
