@@ -9,6 +9,13 @@
 //     each, which the thread that issues the products brings to columns of tensor memory of the stage's own.
 //   * Where W has few tiles of 128 rows, a cluster of up to 8 CTAs shares K.  Each leaves its sums in shared memory, and each adds up
 //     and stores a share of the rows, in the order of the ranks: the result does not depend on timing.
+//
+// Many rows (prompts): bound by the tensor cores.
+//   * 128 rows of x are the M side, 256 (or 128) rows of W the N side, so that a thread of the epilogue has a row of x and a run of columns:
+//     gates beside their ups, whole groups of 32 for 8-bit rows, whole 16-byte pieces to store.
+//   * A CTA an SM takes tile after tile.  One thread asks for the copies, one issues the products, eight warps drain: they take the sums
+//     into registers at once (half of the columns each four warps), give the tensor memory back and work while the next tile is multiplied.
+//
 // Every wait is bounded: a CTA that gives up counts it (janis_mx_timeouts_async), waits for its copies, frees its tensor memory
 // and leaves without a result.  No load here uses cluster multicast.
 #include <cooperative_groups.h>
@@ -35,9 +42,12 @@ struct Out {
     float limit, alpha, up_add;
 };
 
-__device__ __forceinline__ float gated(float gate, float up, const Out& o) {
-    if (o.epi == EPI_GATED_CLAMP) return clamped_gate(gate, up, o.limit, o.alpha, o.up_add);
-    return (o.epi == EPI_GATED_GELU ? gelu_tanh(gate) : gate / (1.0f + expf(-gate))) * up;
+// gelu's tanh form as v / (1 + e^(-2 y)), y = sqrt(2 / pi) (v + 0.044715 v^3): 1 + tanh(y) is 2 / (1 + e^(-2 y)), which loses nothing where
+// tanh comes near -1.  __fdividef is within 2 units in the last place here (and 0 where the divisor has passed 2^126).
+__device__ __forceinline__ float gated(float gate, float up, int epi, const Out& o) {
+    if (epi == EPI_GATED_CLAMP) return clamped_gate(gate, up, o.limit, o.alpha, o.up_add);
+    const float y = epi == EPI_GATED_GELU ? 1.5957691216057308f * fmaf(0.044715f * gate * gate, gate, gate) : gate;
+    return __fdividef(gate, 1.0f + expf(-y)) * up;
 }
 
 constexpr int TILE = 128;                      // rows of W a CTA
@@ -182,7 +192,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             const int cols = share / 2, c0 = n0 / 2 + row0 / 2, all = N / 2, wide = o.codes != nullptr ? padded(all) : all;
             for (int i = threadIdx.x; i < rows * cols; i += 128) {
                 const int m = i / cols, j = i % cols, c = c0 + j, row = row0 + j / 8 * 16 + j % 8;
-                const float v = c < all ? gated(sum_at(m, row), sum_at(m, row + 8), o) : 0.f;
+                const float v = c < all ? gated(sum_at(m, row), sum_at(m, row + 8), o.epi, o) : 0.f;
                 if (o.codes != nullptr) {
                     if (c - lane >= wide) continue;                   // (the whole warp)
                     float big = fabsf(v);
@@ -199,6 +209,215 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         }
     }
     if (split > 1) cluster.sync();                                    // nobody leaves while its sums are read
+}
+
+// ---------------------------------------------------------------------------
+// many rows
+// ---------------------------------------------------------------------------
+constexpr int MANY_THREADS = 384;              // copies; products; two idle warps; two times four warps that drain
+constexpr int X_BYTES = 128 * 128;
+__host__ __device__ constexpr int many_stages(int BN) { return BN == 256 ? 4 : 6; }
+__host__ __device__ constexpr int many_buffers(int BN) { return BN == 256 ? 1 : 2; }      // of sums in tensor memory: 256 columns in all
+constexpr int many_smem(int BN) { return many_stages(BN) * (X_BYTES + BN * 128 + SCALE_BYTES) + 1024; }
+constexpr int M_RUN = 16;                      // tiles of x that are taken with one tile of W after another
+
+__device__ __forceinline__ void tile_at(int i, int m_tiles, int n_tiles, int& m, int& n) {
+    const int run = i / (M_RUN * n_tiles), within = i - run * (M_RUN * n_tiles), height = min(M_RUN, m_tiles - run * M_RUN);
+    n = within / height;
+    m = run * M_RUN + within - n * height;
+}
+
+// `count` values of one row that lie together, at most those that the row has
+template <int COUNT>
+__device__ __forceinline__ void store_run(const uint32_t* v, const Out& o, size_t at, int left, bool vec) {
+    if (o.dtype == JANIS_BF16) {
+        bf16* p = reinterpret_cast<bf16*>(o.values) + at;
+        if (vec) {
+#pragma unroll
+            for (int j = 0; j < COUNT; j += 8)
+                if (j < left) {
+                    float f[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j + e]);
+                    store_eight(p + j, f);
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j)
+                if (j < left) p[j] = from_float<bf16>(__uint_as_float(v[j]));
+        }
+    } else {
+        float* p = reinterpret_cast<float*>(o.values) + at;
+        if (vec) {
+#pragma unroll
+            for (int j = 0; j < COUNT; j += 4)
+                if (j < left) *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j)
+                if (j < left) p[j] = __uint_as_float(v[j]);
+        }
+    }
+}
+
+template <int BN, int EPI>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
+                 const uint8_t* __restrict__ xs, const Out o, int T, int N, int kp, int m_tiles, int n_tiles, int vec) {
+    constexpr int STAGES = many_stages(BN), BUFFERS = many_buffers(BN), STAGE = X_BYTES + BN * 128, W_BLOCKS = BN / BLOCK;
+    constexpr int COLS = BN / 2;                                      // columns of a draining warp
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFFERS];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int blocks = kp / BLOCK, tiles = m_tiles * n_tiles;
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
+    const uint32_t stage0 = (raw + 1023) & ~1023u, scales0 = stage0 + STAGES * STAGE;
+    const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
+    const uint32_t bar_empty = bar_full + 8 * STAGES, bar_sums = bar_full + 16 * STAGES, bar_drained = bar_sums + 8 * BUFFERS;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * STAGES + BUFFERS; ++i) mbar_init(bar_full + 8 * i, 1);
+        for (int i = 0; i < BUFFERS; ++i) mbar_init(bar_drained + 8 * i, 8);
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 0) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), 512);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    int filled = 0;                                                   // stages that copies were asked for (thread 0)
+    grid_dependents_launch();
+
+    if (warp == 0 && lane == 0) {
+        const int w_last = (N - 1) / BLOCK;
+        const auto load_w = [&](int s, int kb, int n0) {
+            mbar_expect_tx(bar_full + 8 * s, X_BYTES + BN * 64 + (1 + W_BLOCKS) * BLOCK_BYTES);
+            tma_load_2d(stage0 + s * STAGE + X_BYTES, &map_w, kb * BLOCK, n0, bar_full + 8 * s);
+#pragma unroll
+            for (int b = 0; b < W_BLOCKS; ++b)                        // (what is past W's rows is zeros whatever their scales)
+                bulk_load(scales0 + s * SCALE_BYTES + (1 + b) * BLOCK_BYTES, ws + ((size_t)min(n0 / BLOCK + b, w_last) * blocks + kb) * BLOCK_BYTES,
+                          BLOCK_BYTES, bar_full + 8 * s);
+        };
+        const auto load_x = [&](int s, int kb, int m) {
+            tma_load_2d(stage0 + s * STAGE, &map_x, kb * BLOCK, m * 128, bar_full + 8 * s);
+            bulk_load(scales0 + s * SCALE_BYTES, xs + ((size_t)m * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
+        };
+        // the weights are constants of the model: the first ones are on their way before x is there
+        const int pre = min(STAGES, blocks);
+        int m, n;
+        tile_at(blockIdx.x, m_tiles, n_tiles, m, n);
+        for (int i = 0; i < pre; ++i) load_w(i, i, n * BN);
+        grid_dependency_wait();
+        for (int i = 0; i < pre; ++i) load_x(i, i, m);
+        filled = pre;
+        bool ok = true;
+        for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
+            tile_at(i, m_tiles, n_tiles, m, n);
+            for (int kb = i == blockIdx.x ? pre : 0; kb < blocks; ++kb, ++filled) {
+                const int s = filled % STAGES;
+                if (filled >= STAGES && !mbar_wait(bar_empty + 8 * s, (filled / STAGES - 1) & 1)) { atomicExch(&failed, 1); ok = false; break; }
+                load_w(s, kb, n * BN);
+                load_x(s, kb, m);
+            }
+        }
+    } else if (warp == 1 && lane == 0) {
+        grid_dependency_wait();
+        int at = 0, turn = 0;
+        bool ok = true;
+        for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x, ++turn) {
+            const int b = turn % BUFFERS;
+            const uint32_t d = tmem + b * BN;
+            if (turn >= BUFFERS && !mbar_wait(bar_drained + 8 * b, (turn / BUFFERS - 1) & 1)) { atomicExch(&failed, 1); break; }
+            fence_after_sync();
+            for (int kb = 0; kb < blocks; ++kb, ++at) {
+                const int s = at % STAGES;
+                if (!mbar_wait(bar_full + 8 * s, (at / STAGES) & 1)) { atomicExch(&failed, 1); ok = false; break; }
+                fence_after_sync();
+                const uint32_t x = stage0 + s * STAGE, w = x + X_BYTES, sc = scales0 + s * SCALE_BYTES;
+                const uint32_t tx = tmem + 256 + s * SCALE_COLS, tw = tx + 4;
+                scales_to_tmem(tx, sc);
+#pragma unroll
+                for (int j = 0; j < W_BLOCKS; ++j) scales_to_tmem(tw + 4 * j, sc + (1 + j) * BLOCK_BYTES);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    umma_block(d, smem_desc(x + g * 32), smem_desc(w + g * 32), block_desc<ROWS>(128, BN, g), tx, tw, (kb > 0 || g > 0) ? 1u : 0u);
+                umma_commit(bar_empty + 8 * s);
+            }
+            umma_commit(bar_sums + 8 * b);
+            if (!ok) mbar_wait(bar_sums + 8 * b, (turn / BUFFERS) & 1);      // (no product is under way when the tensor memory goes)
+        }
+    } else if (warp >= 4) {
+        grid_dependency_wait();
+        const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane;  // (a warp reaches the quarter of tensor memory that its number says)
+        const int cols = EPI == EPI_NONE ? N : N / 2, wide = o.codes != nullptr ? padded(cols) : cols;
+        int turn = 0;
+        for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++turn) {
+            const int b = turn % BUFFERS;
+            int m, n;
+            tile_at(i, m_tiles, n_tiles, m, n);
+            const bool there = mbar_wait_parked(bar_sums + 8 * b, (turn / BUFFERS) & 1, &failed);
+            if (!__all_sync(0xffffffffu, there && *(volatile int*)&failed == 0)) { atomicExch(&failed, 1); break; }
+            fence_after_sync();
+            uint32_t v[COLS];
+#pragma unroll
+            for (int c = 0; c < COLS; c += 32) tmem_load32(v + c, tmem + ((uint32_t)(warp % 4 * 32) << 16) + b * BN + half * COLS + c);
+            tmem_wait_load();
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_drained + 8 * b);
+            const int t = m * 128 + row;
+            if (t >= T) continue;
+            if (EPI == EPI_NONE) {
+                const int c = n * BN + half * COLS;
+                store_run<COLS>(v, o, (size_t)t * N + c, N - c, vec);
+                continue;
+            }
+            const int c = (n * BN + half * COLS) / 2;
+#pragma unroll
+            for (int u = 0; u < COLS / 16; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[u * 8 + j] = __float_as_uint(gated(__uint_as_float(v[u * 16 + j]), __uint_as_float(v[u * 16 + 8 + j]), EPI, o));
+            if (o.codes == nullptr) {
+                store_run<COLS / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
+                continue;
+            }
+#pragma unroll
+            for (int g = 0; g < COLS / 64; ++g) {                     // (columns past the end are products with zeros)
+                float big = 0.f;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) big = larger(big, __uint_as_float(v[g * 32 + j]));
+                const uint32_t byte = scale_byte_e4m3(big);
+                const float inv = inverse_scale(byte);
+                uint32_t q[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t* p = v + g * 32 + j * 4;
+                    q[j] = byte == 255u ? 0u
+                                        : two_e4m3(__uint_as_float(p[0]) * inv, __uint_as_float(p[1]) * inv) |
+                                              two_e4m3(__uint_as_float(p[2]) * inv, __uint_as_float(p[3]) * inv) << 16;
+                }
+                const int cg = c + g * 32;
+                if (cg < wide) {
+                    uint4* to = reinterpret_cast<uint4*>(o.codes + (size_t)t * wide + cg);
+                    to[0] = make_uint4(q[0], q[1], q[2], q[3]);
+                    to[1] = make_uint4(q[4], q[5], q[6], q[7]);
+                    o.scales[scale_at(t, cg / BLOCK, wide / BLOCK) + cg % BLOCK / GROUP] = (uint8_t)byte;
+                }
+            }
+        }
+    }
+    __syncwarp();
+    fence_before_sync();
+    __syncthreads();
+    if (failed != 0 && threadIdx.x == 0) {                            // no copy is under way when the CTA leaves
+        atomicAdd(&g_timeouts, 1);
+        for (int j = filled > STAGES ? filled - STAGES : 0; j < filled; ++j) mbar_wait(bar_full + 8 * (j % STAGES), (j / STAGES) & 1);
+    }
+    if (warp == 0) tmem_free(tmem, 512);
 }
 
 static int sm_count() {
@@ -245,10 +464,43 @@ static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, con
                          xs, o, T, N, kp, NP, split, stages, cols);
 }
 
+template <int BN, int EPI>
+static int many_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
+                        cudaStream_t stream) {
+    const int m_tiles = (T + 127) / 128, n_tiles = o.codes != nullptr ? (padded(N / 2) * 2 + BN - 1) / BN : (N + BN - 1) / BN;
+    if ((long long)m_tiles * n_tiles > 1 << 30) return fail("mx_product: too many tiles");
+    const int cols = EPI == EPI_NONE ? N : N / 2, piece = o.dtype == JANIS_BF16 ? 8 : 4;
+    const int vec = cols % piece == 0 && ((uintptr_t)o.values & 15) == 0;
+    CUtensorMap mw, mx;
+    if (!make_map(&mw, WEIGHTS, wc, N, kp, BN) || !make_map(&mx, ROWS, xc, T, kp, 128))
+        return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
+    static std::once_flag once;
+    static cudaError_t e = cudaSuccess;
+    std::call_once(once, [] { e = cudaFuncSetAttribute(many_rows_kernel<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, many_smem(BN)); });
+    if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
+    const int tiles = m_tiles * n_tiles;
+    return launch_kernel("mx_product", many_rows_kernel<BN, EPI>, dim3(tiles < sm_count() ? tiles : sm_count()), dim3(MANY_THREADS), many_smem(BN),
+                         stream, 1, mw, mx, ws, xs, o, T, N, kp, m_tiles, n_tiles, vec);
+}
+
+template <int BN>
+static int many_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
+                     cudaStream_t stream) {
+    if (o.epi == EPI_NONE) return many_rows_as<BN, EPI_NONE>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_GELU) return many_rows_as<BN, EPI_GATED_GELU>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_SILU) return many_rows_as<BN, EPI_GATED_SILU>(xc, xs, wc, ws, o, T, N, kp, stream);
+    return many_rows_as<BN, EPI_GATED_CLAMP>(xc, xs, wc, ws, o, T, N, kp, stream);
+}
+
 }  // namespace mx
 }  // namespace janis
 
 using namespace janis;
+
+static int g_kernel = 0;
+
+// Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 that of many with 256 and 128 rows of W a tile.  For tests and tuning.
+JANIS_EXPORT void janis_mx_set_kernel(int kernel) { g_kernel = kernel; }
 
 static int g_split = 0, g_stages = 0;
 
@@ -270,7 +522,10 @@ JANIS_EXPORT int janis_mx_product(const uint8_t* xc, const uint8_t* xs, const ui
     if (out_codes == nullptr && out_dtype != JANIS_BF16 && out_dtype != JANIS_F32) return fail("mx_product: unknown dtype %d", out_dtype);
     if (K > 1 << 30) return fail("mx_product: a row has at most 2^30 values, found %d", K);
     const mx::Out o = {out, out_codes, out_scales, out_dtype, epi, limit, alpha, up_add};
-    return mx::few_rows(xc, xs, wc, ws, o, T, N, mx::padded(K), g_split, g_stages, stream);
+    const int kp = mx::padded(K);
+    const int kernel = g_kernel != 0 ? g_kernel : T <= 64 ? 1 : 2;
+    if (kernel == 1) return mx::few_rows(xc, xs, wc, ws, o, T, N, kp, g_split, g_stages, stream);
+    return kernel == 2 ? mx::many_rows<256>(xc, xs, wc, ws, o, T, N, kp, stream) : mx::many_rows<128>(xc, xs, wc, ws, o, T, N, kp, stream);
 }
 
 // The count of given-up waits copied into `host` (pinned memory, two ints, the second always 0) in the order of `stream`.

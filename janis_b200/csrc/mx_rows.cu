@@ -61,6 +61,105 @@ norm_rows_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_part, 
         store_group(i < H ? hr[i] * inv * w_next[i] : 0.f, codes, scales, r, i / GROUP, kp / GROUP, kp);
 }
 
+// Eight values a thread, four threads a group, sixteen a block of 128: codes as 8 bytes, the block's four scales as 4.  Whole warps call it.
+__device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* codes, uint8_t* scales, int r, int j, int blocks, bool live) {
+    float big = fabsf(v[0]);
+#pragma unroll
+    for (int e = 1; e < 8; ++e) big = larger(big, v[e]);
+    big = larger(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = larger(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    const uint32_t byte = scale_byte_e4m3(big);
+    const float inv = inverse_scale(byte);
+    uint32_t four = byte << (8 * (threadIdx.x >> 2 & 3));
+    four |= __shfl_xor_sync(0xffffffffu, four, 4);
+    four |= __shfl_xor_sync(0xffffffffu, four, 8);
+    uint2 q;
+    q.x = two_e4m3(v[0] * inv, v[1] * inv) | two_e4m3(v[2] * inv, v[3] * inv) << 16;
+    q.y = two_e4m3(v[4] * inv, v[5] * inv) | two_e4m3(v[6] * inv, v[7] * inv) << 16;
+    if (byte == 255u) q = make_uint2(0u, 0u);
+    if (!live) return;
+    *reinterpret_cast<uint2*>(codes + ((size_t)r * blocks * BLOCK + (size_t)j * 8)) = q;
+    if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_at(r, j / 16, blocks)) = four;
+}
+
+// The same with the row in registers: thread i takes the pieces of 8 values i, i + blockDim, ... (H a multiple of 8, at most VPT of them a
+// thread), so that each input is read once, 16 bytes at a time, and a row's scales leave four at a time.
+template <typename TR, int VPT>
+__global__ void __launch_bounds__(640)
+norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_part, size_t part_stride, const float* __restrict__ w_post,
+                     float eps_post, const float* __restrict__ w_next, float eps_next, const int* __restrict__ rows,
+                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int H) {
+    __shared__ float scratch[32];
+    const int r = blockIdx.x, pieces = H / 8, all = padded(H) / 8;
+    grid_dependents_launch();
+    float wn[VPT][8], wp[VPT][8];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {                                   // (the norms' weights are constants of the model)
+        const int j = threadIdx.x + k * blockDim.x;
+        if (j < pieces) {
+            load_eight(w_next + j * 8, wn[k]);
+            if (w_post != nullptr) load_eight(w_post + j * 8, wp[k]);
+        }
+    }
+    grid_dependency_wait();
+    float* hr = h + (size_t)(rows ? rows[r] : r) * H;
+    float v[VPT][8], hv[VPT][8];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int j = threadIdx.x + k * blockDim.x;
+        if (j < pieces) {
+            load_eight(hr + j * 8, hv[k]);
+            if (res != nullptr) {
+                const TR* rr = res + (size_t)r * H + j * 8;
+                load_eight(rr, v[k]);
+                for (int p = 1; p < n_part; ++p) {
+                    float more[8];
+                    load_eight(rr + p * part_stride, more);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[k][e] += more[e];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] = hv[k][e] = wn[k][e] = wp[k][e] = 0.f;
+        }
+    }
+    float ss = 0.f;
+    if (res != nullptr) {
+        float inv = 1.f;
+        if (w_post != nullptr) {
+#pragma unroll
+            for (int k = 0; k < VPT; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss = fmaf(v[k][e], v[k][e], ss);
+            ss = block_sum(ss, scratch);
+            inv = 1.0f / sqrtf(ss / (float)H + eps_post);
+            ss = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            const int j = threadIdx.x + k * blockDim.x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hv[k][e] += w_post != nullptr ? v[k][e] * inv * wp[k][e] : v[k][e];
+            if (j < pieces) store_eight(hr + j * 8, hv[k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < VPT; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(hv[k][e], hv[k][e], ss);
+    ss = block_sum(ss, scratch);
+    const float inv = 1.0f / sqrtf(ss / (float)H + eps_next);
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int j = threadIdx.x + k * blockDim.x;
+        if (j - (int)(threadIdx.x & 31) >= all) break;                // (a whole warp)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hv[k][e] = j < pieces ? hv[k][e] * inv * wn[k][e] : 0.f;
+        store_eight_of_group(hv[k], codes, scales, r, j, all / 16, j < all);
+    }
+}
+
 // ---------------------------------------------------------------------------
 // rows as they are, and act(gate) * up over columns that alternate 8 gates, 8 ups (act 0: gelu's tanh form, 1: silu,
 // 2: the clamped gate); a warp a group
@@ -85,6 +184,36 @@ plain_rows_kernel(const T* __restrict__ x, int act, float limit, float alpha, fl
             }
         }
         store_group(v, codes, scales, r, g, groups, kp);
+    }
+}
+
+// the same, eight values a thread (K a multiple of 8, 16-byte pieces)
+template <typename T>
+__global__ void __launch_bounds__(256)
+plain_rows_vec_kernel(const T* __restrict__ x, int act, float limit, float alpha, float up_add, uint8_t* __restrict__ codes,
+                      uint8_t* __restrict__ scales, size_t n_pieces, int K, int kp) {
+    grid_dependents_launch();
+    grid_dependency_wait();
+    const int per_row = kp / 8;
+    for (size_t q = (size_t)blockIdx.x * 256 + threadIdx.x; q - (threadIdx.x & 31) < n_pieces; q += (size_t)gridDim.x * 256) {
+        const bool live = q < n_pieces;
+        const int r = live ? (int)(q / per_row) : 0, j = live ? (int)(q - (size_t)r * per_row) : 0;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        if (live && j * 8 < K) {
+            if (act < 0) {
+                load_eight(x + (size_t)r * K + j * 8, v);
+            } else {
+                float g[8], u[8];
+                load_eight(x + (size_t)r * 2 * K + j * 16, g);
+                load_eight(x + (size_t)r * 2 * K + j * 16 + 8, u);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = act == 2 ? clamped_gate(g[e], u[e], limit, alpha, up_add) : (act == 0 ? gelu_tanh(g[e]) : g[e] / (1.0f + expf(-g[e]))) * u[e];
+            }
+        }
+        store_eight_of_group(v, codes, scales, r, j, kp / BLOCK, live);
     }
 }
 
@@ -124,9 +253,35 @@ values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ sca
     }
 }
 
+template <typename TR>
+static int norm_rows(float* h, const TR* res, int n_part, size_t part_stride, const float* w_post, float eps_post, const float* w_next,
+                     float eps_next, const int* rows, uint8_t* codes, uint8_t* scales, int R, int H, cudaStream_t stream) {
+    const bool vec = H % 8 == 0 && (((uintptr_t)h | (uintptr_t)res | (uintptr_t)w_post | (uintptr_t)w_next) & 15) == 0 && part_stride % 8 == 0;
+    const int pieces = padded(H) / 8;
+    const int vpt = pieces <= 640 ? 1 : pieces <= 1280 ? 2 : 4;
+    if (!vec || pieces > 2560)
+        return launch_kernel("mx_norm_rows", norm_rows_kernel<TR>, dim3(R), dim3(256), 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post,
+                             w_next, eps_next, rows, codes, scales, H);
+    const dim3 block(((pieces + vpt - 1) / vpt + 31) / 32 * 32);
+    return launch_kernel("mx_norm_rows", vpt == 1 ? norm_rows_vec_kernel<TR, 1> : vpt == 2 ? norm_rows_vec_kernel<TR, 2> : norm_rows_vec_kernel<TR, 4>,
+                         dim3(R), block, 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
+}
+
 static int blocks_for(size_t warps) {
     const size_t b = (warps + 7) / 8;
     return (int)(b < 148 * 32 ? b : 148 * 32);
+}
+
+template <typename T>
+static int plain_rows(const T* x, int act, float limit, float alpha, float up_add, uint8_t* codes, uint8_t* scales, int R, int K,
+                      cudaStream_t stream) {
+    const int kp = padded(K);
+    const size_t n_groups = (size_t)R * (kp / GROUP);
+    if (K % 8 == 0 && ((uintptr_t)x & 15) == 0)
+        return launch_kernel("mx_rows", plain_rows_vec_kernel<T>, dim3(blocks_for(n_groups / 8 + 1)), dim3(256), 0, stream, 1, x, act, limit, alpha,
+                             up_add, codes, scales, n_groups * 4, K, kp);
+    return launch_kernel("mx_rows", plain_rows_kernel<T>, dim3(blocks_for(n_groups)), dim3(256), 0, stream, 1, x, act, limit, alpha, up_add, codes,
+                         scales, n_groups, K, kp);
 }
 
 }  // namespace mx
@@ -145,11 +300,9 @@ JANIS_EXPORT int janis_mx_norm_rows(float* h, const void* res, int res_dtype, in
     if (H <= 0) return fail("mx_norm_rows: a row has no values");
     if (res != nullptr && rows != nullptr) return fail("mx_norm_rows: rows are gathered without a residual only");
     if (res_dtype == JANIS_BF16)
-        return launch_kernel("mx_norm_rows", mx::norm_rows_kernel<bf16>, dim3(R), dim3(256), 0, stream, 1, h, (const bf16*)res, n_part,
-                             (size_t)part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
+        return mx::norm_rows(h, (const bf16*)res, n_part, (size_t)part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, R, H, stream);
     if (res_dtype != JANIS_F32) return fail("mx_norm_rows: unknown dtype %d", res_dtype);
-    return launch_kernel("mx_norm_rows", mx::norm_rows_kernel<float>, dim3(R), dim3(256), 0, stream, 1, h, (const float*)res, n_part,
-                         (size_t)part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
+    return mx::norm_rows(h, (const float*)res, n_part, (size_t)part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, R, H, stream);
 }
 
 // act < 0: x [R, K] as it is; otherwise x [R, 2 K] of gates and ups
@@ -159,15 +312,9 @@ JANIS_EXPORT int janis_mx_rows(const void* x, int dtype, int act, float limit, f
     if (K <= 0) return fail("mx_rows: a row has no values");
     if (act > 2) return fail("mx_rows: unknown activation %d", act);
     if (act >= 0 && K % 8) return fail("mx_rows: gates and ups alternate in groups of 8, found %d columns", K);
-    const int kp = mx::padded(K);
-    const size_t n_groups = (size_t)R * (kp / mx::GROUP);
-    const dim3 grid(mx::blocks_for(n_groups));
-    if (dtype == JANIS_BF16)
-        return launch_kernel("mx_rows", mx::plain_rows_kernel<bf16>, grid, dim3(256), 0, stream, 1, (const bf16*)x, act, limit, alpha,
-                             up_add, codes, scales, n_groups, K, kp);
+    if (dtype == JANIS_BF16) return mx::plain_rows((const bf16*)x, act, limit, alpha, up_add, codes, scales, R, K, stream);
     if (dtype != JANIS_F32) return fail("mx_rows: unknown dtype %d", dtype);
-    return launch_kernel("mx_rows", mx::plain_rows_kernel<float>, grid, dim3(256), 0, stream, 1, (const float*)x, act, limit, alpha, up_add,
-                         codes, scales, n_groups, K, kp);
+    return mx::plain_rows((const float*)x, act, limit, alpha, up_add, codes, scales, R, K, stream);
 }
 
 JANIS_EXPORT int janis_mx_weight(const void* w, int dtype, uint8_t* codes, uint8_t* scales, int N, int K, cudaStream_t stream) {

@@ -146,6 +146,12 @@ def mx_set_few(split: int = 0, stages: int = 0) -> None:
     _ops.low_bits().janis_mx_set_few(int(split), int(stages))
 
 
+def mx_set_kernel(kernel: int = 0) -> None:
+    """Fixes the kernel of products: 0 chosen by their sizes, 1 few rows, 2 and 3 many rows with 256 and 128 rows of weights a tile.  For tests
+    and tuning."""
+    _ops.low_bits().janis_mx_set_kernel(int(kernel))
+
+
 def linear_mx(x: MxRows, w: MxWeight, out, epilogue: int = 0, limit: float = 0.0, alpha: float = 1.0, up_add: float = 0.0):
     """out[T, N] = x w^T of 8-bit rows and 4-bit weights, float sums; out bfloat16 or float32.  With a gated epilogue
     (EPI_GATED_GELU, EPI_GATED_SILU, EPI_GATED_CLAMP with its three numbers) the rows of w alternate 8 gates, 8 ups and

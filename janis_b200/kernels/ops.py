@@ -218,6 +218,8 @@ def low_bits():
         lib.janis_mx_product.argtypes = [P, P, P, P, P, I, P, P, I, I, I, I, F, F, F, P]
         lib.janis_mx_set_few.argtypes = [I, I]
         lib.janis_mx_set_few.restype = None
+        lib.janis_mx_set_kernel.argtypes = [I]
+        lib.janis_mx_set_kernel.restype = None
         lib.janis_mx_timeouts_async.argtypes = [P, P]
         lib.janis_mx_set_overlap.argtypes = [I]
         lib.janis_mx_set_overlap.restype = None
@@ -1917,4 +1919,4 @@ def mask_tokens(logits, ids):
 
 
 from . import mx                                                          # noqa: E402  (it uses the helpers above)
-from .mx import MxRows, MxWeight, linear_mx, mx_rows, mx_set_few, mx_weight           # noqa: E402
+from .mx import MxRows, MxWeight, linear_mx, mx_rows, mx_set_few, mx_set_kernel, mx_weight           # noqa: E402
