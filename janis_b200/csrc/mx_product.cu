@@ -64,7 +64,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 1];
     __shared__ uint32_t tmem_slot;
-    __shared__ int failed;
+    __shared__ int failed, asked;                                     // asked: stages that copies were asked for
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = split > 1 ? (int)cg::this_cluster().block_rank() : 0;
     const int n0 = blockIdx.x / split * TILE, t0 = blockIdx.y * NP;
@@ -96,9 +96,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     const uint8_t* w_scales = ws + (size_t)min(n0 / BLOCK, (N - 1) / BLOCK) * blocks * BLOCK_BYTES;
     const uint8_t* x_scales = xs + (size_t)(t0 / BLOCK) * blocks * BLOCK_BYTES;
 
-    int filled = 0;                                                   // stages that copies were asked for (thread 0)
     grid_dependents_launch();
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         // ---- the copies.  The weights are constants of the model: the first tiles of W are on their way before this kernel
         // waits for the one that makes x.
         const int bytes = A_PACKED + NP * 128 + (1 + x_blocks) * BLOCK_BYTES;
@@ -118,13 +117,15 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         for (int i = 0; i < pre; ++i) load_w(i, i);
         grid_dependency_wait();
         for (int i = 0; i < pre; ++i) load_x(i, i);
-        for (filled = pre; filled < nk; ++filled) {
+        int filled = pre;
+        for (; filled < nk; ++filled) {
             const int s = filled % stages;
             if (!mbar_wait(bar_empty + 8 * s, (filled / stages - 1) & 1)) { atomicExch(&failed, 1); break; }
             load_w(filled, s);
             load_x(filled, s);
         }
-    } else if (warp == 1 && lane == 0) {
+        asked = filled;
+    } else if (warp == 1 && elect_one()) {
         // ---- the thread that issues the products
         grid_dependency_wait();
         for (int i = 0; i < nk; ++i) {
@@ -149,7 +150,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     ok = __syncthreads_and(ok ? 1 : 0) && failed == 0;
     fence_after_sync();
     if (!ok && threadIdx.x == 0)                                      // no copy is under way when the CTA leaves
-        for (int j = filled > stages ? filled - stages : 0; j < filled; ++j) mbar_wait(bar_full + 8 * (j % stages), (j / stages) & 1);
+        for (int j = asked > stages ? asked - stages : 0; j < asked; ++j) mbar_wait(bar_full + 8 * (j % stages), (j / stages) & 1);
 
     // ---- sums of row (32 * warp + lane) of the tile of W
     for (int c = 0; c < NP; c += 16) {
@@ -269,7 +270,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFFERS];
     __shared__ uint32_t tmem_slot;
-    __shared__ int failed;
+    __shared__ int failed, asked;                                     // asked: stages that copies were asked for
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = kp / BLOCK, tiles = m_tiles * n_tiles;
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
@@ -288,10 +289,9 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
-    int filled = 0;                                                   // stages that copies were asked for (thread 0)
     grid_dependents_launch();
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         const int w_last = (N - 1) / BLOCK;
         const auto load_w = [&](int s, int kb, int n0) {
             mbar_expect_tx(bar_full + 8 * s, X_BYTES + BN * 64 + (1 + W_BLOCKS) * BLOCK_BYTES);
@@ -312,7 +312,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         for (int i = 0; i < pre; ++i) load_w(i, i, n * BN);
         grid_dependency_wait();
         for (int i = 0; i < pre; ++i) load_x(i, i, m);
-        filled = pre;
+        int filled = pre;
         bool ok = true;
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
             tile_at(i, m_tiles, n_tiles, m, n);
@@ -323,7 +323,8 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 load_x(s, kb, m);
             }
         }
-    } else if (warp == 1 && lane == 0) {
+        asked = filled;
+    } else if (warp == 1 && elect_one()) {
         grid_dependency_wait();
         int at = 0, turn = 0;
         bool ok = true;
@@ -415,7 +416,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     __syncthreads();
     if (failed != 0 && threadIdx.x == 0) {                            // no copy is under way when the CTA leaves
         atomicAdd(&g_timeouts, 1);
-        for (int j = filled > STAGES ? filled - STAGES : 0; j < filled; ++j) mbar_wait(bar_full + 8 * (j % STAGES), (j / STAGES) & 1);
+        for (int j = asked > STAGES ? asked - STAGES : 0; j < asked; ++j) mbar_wait(bar_full + 8 * (j % STAGES), (j / STAGES) & 1);
     }
     if (warp == 0) tmem_free(tmem, 512);
 }
