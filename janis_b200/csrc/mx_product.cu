@@ -7,8 +7,9 @@
 //     128 rows of W are the M side, one a lane of tensor memory; the rows of x, padded to a multiple of 16, the N side.
 //   * A stage is 128 values of K: 8 KB of W (16 KB once the copy engine has spread it), the rows of x, and a block of scales of
 //     each, which the thread that issues the products brings to columns of tensor memory of the stage's own.
-//   * Where W has few tiles of 128 rows, a cluster of up to 8 CTAs shares K.  Each leaves its sums in shared memory, and each adds up
-//     and stores a share of the rows, in the order of the ranks: the result does not depend on timing.
+//   * Where W has few tiles of 128 rows, a cluster of up to 8 CTAs shares K.  Each sends its sums to the CTAs that add them up, a share
+//     of the rows each, in the order of the ranks: the result does not depend on timing.  The sums are counted in by an mbarrier; nobody
+//     waits for anybody else at the end.
 //
 // Many rows (prompts): bound by the tensor cores.
 //   * 128 rows of x are the M side, 256 (or 128) rows of W the N side, so that a thread of the epilogue has a row of x and a run of columns:
@@ -56,41 +57,51 @@ constexpr int MAX_STAGES = 11;
 constexpr int MAX_ROWS = 256;                  // rows of x a CTA
 constexpr int SCALE_BYTES = 3 * BLOCK_BYTES;   // of a stage: a block of W's, one or two of x's
 constexpr int SCALE_COLS = 12;
-constexpr int few_smem(int stages, int NP) { return stages * (A_BYTES + NP * 128 + SCALE_BYTES) + 1024; }
+constexpr int few_smem(int stages, int NP, int split) {
+    return stages * (A_BYTES + NP * 128 + SCALE_BYTES) + 1024 + (split > 1 ? NP * TILE * 4 : 0);
+}
 
+template <int SPLIT>
 __global__ void __launch_bounds__(128)
 few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
-                const uint8_t* __restrict__ xs, const Out o, int T, int N, int kp, int NP, int split, int stages, int tmem_cols) {
+                const uint8_t* __restrict__ xs, const Out o, int T, int N, int kp, int NP, int stages, int tmem_cols) {
+    constexpr int SHARE = TILE / SPLIT;                              // rows of the tile that this CTA adds up and stores
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 1];
+    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed, asked;                                     // asked: stages that copies were asked for
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = split > 1 ? (int)cg::this_cluster().block_rank() : 0;
-    const int n0 = blockIdx.x / split * TILE, t0 = blockIdx.y * NP;
-    const int blocks = kp / BLOCK;
+    const int rank = SPLIT > 1 ? (int)cg::this_cluster().block_rank() : 0;
+    const int n0 = blockIdx.x / SPLIT * TILE, t0 = blockIdx.y * NP;
+    const int blocks = kp / BLOCK, rows = min(T - t0, NP);
 
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
     const uint32_t stage0 = (raw + 1023) & ~1023u;                   // swizzle atoms want 1024-byte alignment
-    float* sums = reinterpret_cast<float*>(smem_raw + (stage0 - raw));      // [NP][TILE], once the stages are idle
     const int stage_bytes = A_BYTES + NP * 128;
     const uint32_t scales0 = stage0 + stages * stage_bytes;
+    // [SPLIT][rows][SHARE] sums: behind the stages where others write them, over the idle stages where this CTA does
+    const uint32_t sums0 = SPLIT > 1 ? scales0 + stages * SCALE_BYTES : stage0;
+    float* sums = reinterpret_cast<float*>(smem_raw + (sums0 - raw));
     const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
-    const uint32_t bar_empty = bar_full + 8 * stages, bar_done = bar_full + 16 * stages;
+    const uint32_t bar_empty = bar_full + 8 * MAX_STAGES, bar_done = bar_full + 16 * MAX_STAGES, bar_sums = bar_done + 8;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * stages + 1; ++i) mbar_init(bar_full + 8 * i, 1);
+        for (int i = 0; i < stages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
+        mbar_init(bar_done, 1);
+        mbar_init(bar_sums, 1);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        if (SPLIT > 1) mbar_expect_tx(bar_sums, rows * TILE * 4);
     }
     if (warp == 0) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), tmem_cols);
     fence_before_sync();
     __syncthreads();
+    if (SPLIT > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
     fence_after_sync();
     const uint32_t tmem = tmem_slot;
 
-    // this CTA's share of K: value blocks rank, rank + split, ...
-    const int nk = (blocks - rank + split - 1) / split;
+    // this CTA's share of K: value blocks rank, rank + SPLIT, ...
+    const int nk = (blocks - rank + SPLIT - 1) / SPLIT;
     const int x_blocks = NP > BLOCK && t0 + BLOCK < T ? 2 : 1;       // blocks of x's scales that are there
     // (a tile past W's rows, which only makes the padding of 8-bit rows, finds zeros there whatever their scales)
     const uint8_t* w_scales = ws + (size_t)min(n0 / BLOCK, (N - 1) / BLOCK) * blocks * BLOCK_BYTES;
@@ -101,36 +112,36 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         // ---- the copies.  The weights are constants of the model: the first tiles of W are on their way before this kernel
         // waits for the one that makes x.
         const int bytes = A_PACKED + NP * 128 + (1 + x_blocks) * BLOCK_BYTES;
-        const auto load_w = [&](int i, int s) {
+        const auto load_w = [&](int kb, int s) {
             mbar_expect_tx(bar_full + 8 * s, bytes);
-            const int kb = rank + i * split;
             tma_load_2d(stage0 + s * stage_bytes, &map_w, kb * BLOCK, n0, bar_full + 8 * s);
             bulk_load(scales0 + s * SCALE_BYTES, w_scales + (size_t)kb * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
         };
-        const auto load_x = [&](int i, int s) {
-            const int kb = rank + i * split;
+        const auto load_x = [&](int kb, int s) {
             tma_load_2d(stage0 + s * stage_bytes + A_BYTES, &map_x, kb * BLOCK, t0, bar_full + 8 * s);
             for (int b = 0; b < x_blocks; ++b)
                 bulk_load(scales0 + s * SCALE_BYTES + (1 + b) * BLOCK_BYTES, x_scales + ((size_t)b * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
         };
         const int pre = nk < stages ? nk : stages;
-        for (int i = 0; i < pre; ++i) load_w(i, i);
+        for (int i = 0; i < pre; ++i) load_w(rank + i * SPLIT, i);
         grid_dependency_wait();
-        for (int i = 0; i < pre; ++i) load_x(i, i);
-        int filled = pre;
+        for (int i = 0; i < pre; ++i) load_x(rank + i * SPLIT, i);
+        int filled = pre, s = 0;
+        uint32_t phase = 0;
         for (; filled < nk; ++filled) {
-            const int s = filled % stages;
-            if (!mbar_wait(bar_empty + 8 * s, (filled / stages - 1) & 1)) { atomicExch(&failed, 1); break; }
-            load_w(filled, s);
-            load_x(filled, s);
+            if (!mbar_wait(bar_empty + 8 * s, phase)) { atomicExch(&failed, 1); break; }
+            load_w(rank + filled * SPLIT, s);
+            load_x(rank + filled * SPLIT, s);
+            if (++s == stages) { s = 0; phase ^= 1; }
         }
         asked = filled;
     } else if (warp == 1 && elect_one()) {
         // ---- the thread that issues the products
         grid_dependency_wait();
+        int s = 0;
+        uint32_t phase = 0;
         for (int i = 0; i < nk; ++i) {
-            const int s = i % stages;
-            if (!mbar_wait(bar_full + 8 * s, (i / stages) & 1)) { atomicExch(&failed, 1); break; }
+            if (!mbar_wait(bar_full + 8 * s, phase)) { atomicExch(&failed, 1); break; }
             fence_after_sync();
             const uint32_t a = stage0 + s * stage_bytes, b = a + A_BYTES, sc = scales0 + s * SCALE_BYTES;
             const uint32_t ta = tmem + NP + s * SCALE_COLS, tb = ta + 4;
@@ -140,6 +151,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             for (int g = 0; g < 4; ++g)                               // 32 bytes further along the swizzled row
                 umma_block(tmem, smem_desc(a + g * 32), smem_desc(b + g * 32), block_desc<WEIGHTS>(TILE, NP, g), ta, tb, (i > 0 || g > 0) ? 1u : 0u);
             umma_commit(bar_empty + 8 * s);                           // the stage is free once these have read it
+            if (++s == stages) { s = 0; phase ^= 1; }
         }
         umma_commit(bar_done);                                        // all products of this CTA have finished
     } else {
@@ -151,65 +163,79 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     fence_after_sync();
     if (!ok && threadIdx.x == 0)                                      // no copy is under way when the CTA leaves
         for (int j = asked > stages ? asked - stages : 0; j < asked; ++j) mbar_wait(bar_full + 8 * (j % stages), (j / stages) & 1);
+    if (SPLIT > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // everybody's barriers are there
 
-    // ---- sums of row (32 * warp + lane) of the tile of W
-    for (int c = 0; c < NP; c += 16) {
+    // ---- sums of row (32 * warp + lane) of the tile of W, to the CTA that adds them up
+    const uint32_t mine = sums0 + (uint32_t)(rank * rows * SHARE + threadIdx.x % SHARE) * 4;
+    uint32_t there = mine, there_bar = bar_sums;
+    if (SPLIT > 1) {
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there) : "r"(mine), "r"((uint32_t)threadIdx.x / SHARE));
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there_bar) : "r"(bar_sums), "r"((uint32_t)threadIdx.x / SHARE));
+    }
+    for (int c = 0; c < rows; c += 16) {
         uint32_t r[16];
         tmem_load16(r, tmem + ((uint32_t)(warp * 32) << 16) + c);
         tmem_wait_load();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sums[(c + j) * TILE + threadIdx.x] = __uint_as_float(r[j]);
-    }
-    fence_before_sync();
-    __syncthreads();
-    if (warp == 0) tmem_free(tmem, tmem_cols);
-    if (!ok && threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
-    cg::cluster_group cluster = cg::this_cluster();
-    const float* theirs[8];
-    if (split > 1) {
-        cluster.sync();
-        for (int r = 0; r < split; ++r) theirs[r] = cluster.map_shared_rank(sums, r);
-    } else {
-        theirs[0] = sums;
-    }
-    const auto sum_at = [&](int m, int row) {
-        float v = theirs[0][m * TILE + row];
-        for (int r = 1; r < split; ++r) v += theirs[r][m * TILE + row];
-        return v;
-    };
-    // ---- this CTA's share: rows [row0, row0 + share) of the tile, all rows of x
-    const int rows = T - t0 < NP ? T - t0 : NP, share = TILE / split, row0 = rank * share;
-    if (ok) {
-        if (o.epi == EPI_NONE) {
-            for (int i = threadIdx.x; i < rows * share; i += 128) {
-                const int m = i / share, row = row0 + i % share, n = n0 + row;
-                if (n >= N) continue;
-                const float v = sum_at(m, row);
-                if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * N + n] = from_float<bf16>(v);
-                else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * N + n] = v;
-            }
-        } else {
-            // a gate's up stands 8 rows behind it; for 8-bit rows a warp has the 32 columns of a group (the share is 64 rows at least)
-            const int cols = share / 2, c0 = n0 / 2 + row0 / 2, all = N / 2, wide = o.codes != nullptr ? padded(all) : all;
-            for (int i = threadIdx.x; i < rows * cols; i += 128) {
-                const int m = i / cols, j = i % cols, c = c0 + j, row = row0 + j / 8 * 16 + j % 8;
-                const float v = c < all ? gated(sum_at(m, row), sum_at(m, row + 8), o.epi, o) : 0.f;
-                if (o.codes != nullptr) {
-                    if (c - lane >= wide) continue;                   // (the whole warp)
-                    float big = fabsf(v);
-#pragma unroll
-                    for (int s = 16; s > 0; s >>= 1) big = larger(big, __shfl_xor_sync(0xffffffffu, big, s));
-                    const uint32_t byte = scale_byte_e4m3(big);
-                    o.codes[(size_t)(t0 + m) * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v * inverse_scale(byte), 0.f);
-                    if (lane == 0) o.scales[scale_at(t0 + m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
-                } else if (c < all) {
-                    if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * all + c] = from_float<bf16>(v);
-                    else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * all + c] = v;
-                }
-            }
+        for (int j = 0; j < 16; ++j) {
+            if (c + j >= rows) break;
+            if (SPLIT > 1)
+                asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];\n" ::"r"(there + (uint32_t)(c + j) * SHARE * 4),
+                             "r"(r[j]), "r"(there_bar)
+                             : "memory");
+            else
+                sums[(c + j) * TILE + threadIdx.x] = __uint_as_float(r[j]);
         }
     }
-    if (split > 1) cluster.sync();                                    // nobody leaves while its sums are read
+    fence_before_sync();
+    if (SPLIT > 1) {
+        // (others may be at their own waits' limits: this CTA's memory has to outlast what they send)
+        bool all = false;
+        for (int i = 0; i < 8 && !all; ++i) all = mbar_wait(bar_sums, 0);
+        ok = ok && all;
+    }
+    ok = __syncthreads_and(ok ? 1 : 0);
+    if (warp == 0) tmem_free(tmem, tmem_cols);
+    if (!ok) {
+        if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
+        return;
+    }
+    const auto sum_at = [&](int m, int row) {                         // in the order of the ranks
+        float v = sums[m * SHARE + row];
+#pragma unroll
+        for (int r = 1; r < SPLIT; ++r) v += sums[(r * rows + m) * SHARE + row];
+        return v;
+    };
+    const int row0 = n0 + rank * SHARE;
+    if (o.epi == EPI_NONE) {
+        const int row = threadIdx.x % SHARE, n = row0 + row;
+        if (n >= N) return;
+        for (int m = threadIdx.x / SHARE; m < rows; m += SPLIT) {
+            const float v = sum_at(m, row);
+            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * N + n] = from_float<bf16>(v);
+            else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * N + n] = v;
+        }
+        return;
+    }
+    // a gate's up stands 8 rows behind it; for 8-bit rows a warp has the 32 columns of a group (SHARE is 64 at least)
+    constexpr int COLS = SHARE / 2;
+    const int j = threadIdx.x % COLS, c = row0 / 2 + j, row = j / 8 * 16 + j % 8;
+    const int all = N / 2, wide = o.codes != nullptr ? padded(all) : all;
+    if (c >= wide) return;                                            // (for 8-bit rows a whole warp)
+    for (int m = threadIdx.x / COLS; m < rows; m += 128 / COLS) {
+        const float v = c < all ? gated(sum_at(m, row), sum_at(m, row + 8), o.epi, o) : 0.f;
+        if (o.codes != nullptr) {
+            float big = fabsf(v);
+#pragma unroll
+            for (int s = 16; s > 0; s >>= 1) big = larger(big, __shfl_xor_sync(0xffffffffu, big, s));
+            const uint32_t byte = scale_byte_e4m3(big);
+            o.codes[(size_t)(t0 + m) * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v * inverse_scale(byte), 0.f);
+            if (lane == 0) o.scales[scale_at(t0 + m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
+        } else if (c < all) {
+            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * all + c] = from_float<bf16>(v);
+            else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * all + c] = v;
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -410,6 +436,8 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 }
             }
         }
+    } else {
+        grid_dependency_wait();
     }
     __syncwarp();
     fence_before_sync();
@@ -441,28 +469,33 @@ static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, con
         split = 1;
         while (split < most_split && tiles * t_tiles * split * 2 <= sm_count() && blocks >= split * 2) split *= 2;
     }
-    if (split > most_split || split > blocks) return fail("mx_product: a split of %d is not possible here", split);
+    if (split > most_split || split > blocks || (split & (split - 1)) != 0) return fail("mx_product: a split of %d is not possible here", split);
+    const int most = 227 * 1024 - 512;
     if (stages == 0) {
         const int per_sm = (tiles * t_tiles * split + sm_count() - 1) / sm_count();
-        stages = (227 * 1024 / (per_sm >= 2 ? 2 : 1) - 2048) / (A_BYTES + NP * 128 + SCALE_BYTES);
-        if (NP > 128 && stages < 4) stages = 4;                       // (the sums of 256 rows leave through four stages)
+        stages = ((per_sm >= 2 ? 113 * 1024 : most) - 1024 - (split > 1 ? NP * TILE * 4 : 0)) / (A_BYTES + NP * 128 + SCALE_BYTES);
         const int share = (blocks + split - 1) / split;
         if (stages > share) stages = share;
-        while (few_smem(stages, NP) < NP * TILE * 4 + 1024) ++stages;
+        if (stages > MAX_STAGES) stages = MAX_STAGES;
+        while (split == 1 && stages * (A_BYTES + NP * 128) < NP * TILE * 4) ++stages;      // (the sums leave through them)
     }
-    if (stages < 1 || stages > MAX_STAGES || few_smem(stages, NP) > 227 * 1024 - 512 || few_smem(stages, NP) < NP * TILE * 4 + 1024)
+    if (stages < 1 || stages > MAX_STAGES || few_smem(stages, NP, split) > most || (split == 1 && stages * (A_BYTES + NP * 128) < NP * TILE * 4))
         return fail("mx_product: %d stages of %d rows do not fit", stages, NP);
     int cols = 32;
     while (cols < NP + stages * SCALE_COLS) cols *= 2;
     CUtensorMap mw, mx;
     if (!make_map(&mw, WEIGHTS, wc, N, kp, TILE) || !make_map(&mx, ROWS, xc, T, kp, NP))
         return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
+    const auto kernel = split == 1 ? few_rows_kernel<1> : split == 2 ? few_rows_kernel<2> : split == 4 ? few_rows_kernel<4> : few_rows_kernel<8>;
     static std::once_flag once;
     static cudaError_t e = cudaSuccess;
-    std::call_once(once, [] { e = cudaFuncSetAttribute(few_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512); });
+    std::call_once(once, [] {
+        for (const auto k : {few_rows_kernel<1>, few_rows_kernel<2>, few_rows_kernel<4>, few_rows_kernel<8>})
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512);
+    });
     if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
-    return launch_kernel("mx_product", few_rows_kernel, dim3(tiles * split, t_tiles), dim3(128), few_smem(stages, NP), stream, split, mw, mx, ws,
-                         xs, o, T, N, kp, NP, split, stages, cols);
+    return launch_kernel("mx_product", kernel, dim3(tiles * split, t_tiles), dim3(128), few_smem(stages, NP, split), stream, split, mw, mx, ws, xs, o,
+                         T, N, kp, NP, stages, cols);
 }
 
 template <int BN, int EPI>
