@@ -449,6 +449,188 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     if (warp == 0) tmem_free(tmem, 512);
 }
 
+// ---------------------------------------------------------------------------
+// many rows of which there are not enough tiles for the SMs: a cluster shares K
+// ---------------------------------------------------------------------------
+constexpr int SHARED_STAGES = 4, SHARED_STAGE = X_BYTES + A_BYTES, SHARED_SCALES = 2 * BLOCK_BYTES;
+constexpr int SHARED_SMEM = SHARED_STAGES * (SHARED_STAGE + SHARED_SCALES) + 128 * 128 * 4 + 1024;
+
+// where 16 bytes of sums (columns 4 c .. 4 c + 3 of row `row`) of a rank stand in the CTA that adds them up: the columns are turned by the row, so
+// that 32 rows that send the same columns do not meet in the same banks
+template <int SPLIT>
+__device__ __forceinline__ uint32_t sums_at(int rank, int row, int c) {
+    return (uint32_t)((rank * (128 / SPLIT) + row) * 512 + ((c ^ (row & 31)) << 4));
+}
+
+template <int SPLIT, int EPI>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
+                   const uint8_t* __restrict__ xs, const Out o, int T, int N, int kp, int m_tiles, int vec) {
+    constexpr int ROWS = 128 / SPLIT, RUN = 64 / SPLIT;               // rows that a CTA adds up; columns of a row that a thread does
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * SHARED_STAGES + 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed, asked;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cg::this_cluster().block_rank(), tile = blockIdx.x / SPLIT, m = tile % m_tiles, n = tile / m_tiles;
+    const int blocks = kp / BLOCK, nk = (blocks - rank + SPLIT - 1) / SPLIT;
+    const int rows = min(T - m * 128, 128), mine = min(max(rows - rank * ROWS, 0), ROWS);
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
+    const uint32_t stage0 = (raw + 1023) & ~1023u, scales0 = stage0 + SHARED_STAGES * SHARED_STAGE, sums0 = scales0 + SHARED_STAGES * SHARED_SCALES;
+    const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
+    const uint32_t bar_empty = bar_full + 8 * SHARED_STAGES, bar_done = bar_full + 16 * SHARED_STAGES, bar_sums = bar_done + 8;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * SHARED_STAGES + 2; ++i) mbar_init(bar_full + 8 * i, 1);
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        mbar_expect_tx(bar_sums, SPLIT * mine * 512);
+    }
+    if (warp == 0) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), 256);
+    fence_before_sync();
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory");
+    fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    grid_dependents_launch();
+
+    if (warp == 0 && elect_one()) {
+        const uint8_t* w_scales = ws + (size_t)min(n, (N - 1) / BLOCK) * blocks * BLOCK_BYTES;
+        const uint8_t* x_scales = xs + (size_t)m * blocks * BLOCK_BYTES;
+        const auto load_w = [&](int kb, int s) {
+            mbar_expect_tx(bar_full + 8 * s, X_BYTES + A_PACKED + 2 * BLOCK_BYTES);
+            tma_load_2d(stage0 + s * SHARED_STAGE + X_BYTES, &map_w, kb * BLOCK, n * 128, bar_full + 8 * s);
+            bulk_load(scales0 + s * SHARED_SCALES + BLOCK_BYTES, w_scales + (size_t)kb * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
+        };
+        const auto load_x = [&](int kb, int s) {
+            tma_load_2d(stage0 + s * SHARED_STAGE, &map_x, kb * BLOCK, m * 128, bar_full + 8 * s);
+            bulk_load(scales0 + s * SHARED_SCALES, x_scales + (size_t)kb * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
+        };
+        const int pre = min(SHARED_STAGES, nk);
+        for (int i = 0; i < pre; ++i) load_w(rank + i * SPLIT, i);
+        grid_dependency_wait();
+        for (int i = 0; i < pre; ++i) load_x(rank + i * SPLIT, i);
+        int filled = pre;
+        for (; filled < nk; ++filled) {
+            const int s = filled % SHARED_STAGES;
+            if (!mbar_wait(bar_empty + 8 * s, (filled / SHARED_STAGES - 1) & 1)) { atomicExch(&failed, 1); break; }
+            load_w(rank + filled * SPLIT, s);
+            load_x(rank + filled * SPLIT, s);
+        }
+        asked = filled;
+    } else if (warp == 1 && elect_one()) {
+        grid_dependency_wait();
+        for (int i = 0; i < nk; ++i) {
+            const int s = i % SHARED_STAGES;
+            if (!mbar_wait(bar_full + 8 * s, (i / SHARED_STAGES) & 1)) { atomicExch(&failed, 1); break; }
+            fence_after_sync();
+            const uint32_t x = stage0 + s * SHARED_STAGE, w = x + X_BYTES, sc = scales0 + s * SHARED_SCALES, tx = tmem + 128 + s * 8, tw = tx + 4;
+            scales_to_tmem(tx, sc);
+            scales_to_tmem(tw, sc + BLOCK_BYTES);
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                umma_block(tmem, smem_desc(x + g * 32), smem_desc(w + g * 32), block_desc<mx::ROWS>(128, 128, g), tx, tw, (i > 0 || g > 0) ? 1u : 0u);
+            umma_commit(bar_empty + 8 * s);
+        }
+        umma_commit(bar_done);
+    } else {
+        grid_dependency_wait();
+    }
+    __syncwarp();
+    bool ok = mbar_wait_parked(bar_done, 0, &failed);
+    ok = __syncthreads_and(ok ? 1 : 0) && failed == 0;
+    fence_after_sync();
+    if (!ok && threadIdx.x == 0)                                      // no copy is under way when the CTA leaves
+        for (int j = asked > SHARED_STAGES ? asked - SHARED_STAGES : 0; j < asked; ++j)
+            mbar_wait(bar_full + 8 * (j % SHARED_STAGES), (j / SHARED_STAGES) & 1);
+    asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // everybody's barriers are there
+
+    if (warp >= 4) {
+        const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane, owner = row / ROWS;
+        uint32_t there, there_bar;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there) : "r"(sums0), "r"((uint32_t)owner));
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there_bar) : "r"(bar_sums), "r"((uint32_t)owner));
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+            uint32_t v[32];
+            tmem_load32(v, tmem + ((uint32_t)(warp % 4 * 32) << 16) + half * 64 + c);
+            tmem_wait_load();
+            if (row < rows) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 4)
+                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];\n" ::"r"(
+                                     there + sums_at<SPLIT>(rank, row % ROWS, (half * 64 + c + j) / 4)),
+                                 "r"(v[j]), "r"(v[j + 1]), "r"(v[j + 2]), "r"(v[j + 3]), "r"(there_bar)
+                                 : "memory");
+            }
+        }
+    }
+    fence_before_sync();
+    {
+        // (others may be at their own waits' limits: this CTA's memory has to outlast what they send)
+        bool all = false;
+        for (int i = 0; i < 8 && !all; ++i) all = mbar_wait(bar_sums, 0);
+        ok = ok && all;
+    }
+    ok = __syncthreads_and(ok ? 1 : 0);
+    if (warp == 0) tmem_free(tmem, 256);
+    if (!ok) {
+        if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
+        return;
+    }
+    if (warp < 4) return;
+    // ---- a run of one row's columns, added up in the order of the ranks
+    const int id = threadIdx.x - 128, row = id / (2 * SPLIT), c0 = id % (2 * SPLIT) * RUN, t = m * 128 + rank * ROWS + row;
+    const bool live = row < mine;
+    uint32_t v[RUN];
+#pragma unroll
+    for (int c = 0; c < RUN; c += 4) {
+        float f[4];
+#pragma unroll
+        for (int r = 0; r < SPLIT; ++r) {
+            float g[4];
+            Vec16<float>::load(reinterpret_cast<const float*>(smem_raw + (sums0 - raw) + sums_at<SPLIT>(r, row, (c0 + c) / 4)), g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = r == 0 ? g[e] : f[e] + g[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] = __float_as_uint(f[e]);
+    }
+    if (EPI == EPI_NONE) {
+        if (live) store_run<RUN>(v, o, (size_t)t * N + n * 128 + c0, N - n * 128 - c0, vec);
+        return;
+    }
+    if constexpr (EPI != EPI_NONE && RUN >= 16) {
+        const int cols = N / 2, wide = o.codes != nullptr ? padded(cols) : cols, c = (n * 128 + c0) / 2;
+#pragma unroll
+        for (int u = 0; u < RUN / 16; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[u * 8 + j] = __float_as_uint(gated(__uint_as_float(v[u * 16 + j]), __uint_as_float(v[u * 16 + 8 + j]), EPI, o));
+        if (o.codes == nullptr) {
+            if (live) store_run<RUN / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
+            return;
+        }
+        constexpr int HELD = RUN / 2;                                 // columns of a thread: 16 or 8 of a group of 32
+        float big = 0.f;
+#pragma unroll
+        for (int j = 0; j < HELD; ++j) big = larger(big, __uint_as_float(v[j]));
+#pragma unroll
+        for (int l = 1; l < 32 / HELD; l *= 2) big = larger(big, __shfl_xor_sync(0xffffffffu, big, l));
+        const uint32_t byte = scale_byte_e4m3(big);
+        const float inv = inverse_scale(byte);
+        if (!live || c >= wide) return;
+#pragma unroll
+        for (int j = 0; j < HELD; j += 4) {
+            const uint32_t q = byte == 255u ? 0u
+                                            : two_e4m3(__uint_as_float(v[j]) * inv, __uint_as_float(v[j + 1]) * inv) |
+                                                  two_e4m3(__uint_as_float(v[j + 2]) * inv, __uint_as_float(v[j + 3]) * inv) << 16;
+            *reinterpret_cast<uint32_t*>(o.codes + (size_t)t * wide + c + j) = q;
+        }
+        if (c % GROUP == 0) o.scales[scale_at(t, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
+    }
+}
+
 static int sm_count() {
     static int sms = 0;
     if (sms == 0) {
@@ -466,17 +648,26 @@ static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, con
     const int tiles = o.codes != nullptr ? padded(N / 2) / (TILE / 2) : (N + TILE - 1) / TILE, blocks = kp / BLOCK, t_tiles = (T + NP - 1) / NP;
     const int most_split = o.codes != nullptr ? 2 : 8;                // (a group of 8-bit rows lies within a CTA's share)
     if (split == 0) {
+        // K is shared while all CTAs are resident, two an SM, and keep four blocks each.  A cluster lies within a GPC, of whose 16 to 18
+        // SMs four clusters of 8 take all: 32 in all, or 48 of three CTAs an SM, which pay where K is long only.  One row, us with 1, 2, 4,
+        // 8 CTAs: 2,304 x 2,048 5.3, 3.6, 2.9, 3.3; 4,096 x 2,304 5.8, 3.8, 3.4, 4.2; 2,304 x 9,216 18, 10, 6.4, 4.8; 18,432 x 2,304 7.2, 6.1;
+        // 4,608 x 4,096 -, -, 4.4, 4.8 (36 tiles); 4,608 x 36,864 66, 34, 22, 20 (36 tiles).
+        const long long ctas = (long long)tiles * t_tiles;
         split = 1;
-        while (split < most_split && tiles * t_tiles * split * 2 <= sm_count() && blocks >= split * 2) split *= 2;
+        while (split < most_split && ctas * split * 2 <= (NP > 64 ? 1 : 2) * sm_count() && blocks >= split * 2 * 4 && (split < 4 || ctas <= 32)) split *= 2;
+        if (split == 4 && most_split == 8 && NP <= 32 && ctas > 32 && ctas <= 48 && blocks >= 128) split = 8;
     }
     if (split > most_split || split > blocks || (split & (split - 1)) != 0) return fail("mx_product: a split of %d is not possible here", split);
     const int most = 227 * 1024 - 512;
     if (stages == 0) {
-        const int per_sm = (tiles * t_tiles * split + sm_count() - 1) / sm_count();
-        stages = ((per_sm >= 2 ? 113 * 1024 : most) - 1024 - (split > 1 ? NP * TILE * 4 : 0)) / (A_BYTES + NP * 128 + SCALE_BYTES);
+        // a ring as deep as the SM's memory allows for the CTAs that share it
+        const long long ctas = (long long)tiles * t_tiles;
+        const int room = split == 8 && NP <= 32 && ctas > 32 ? 74 * 1024 : (split > 1 && NP <= 64) || ctas > sm_count() ? 113 * 1024 : most;
+        stages = (room - 1024 - (split > 1 ? NP * TILE * 4 : 0)) / (A_BYTES + NP * 128 + SCALE_BYTES);
         const int share = (blocks + split - 1) / split;
         if (stages > share) stages = share;
         if (stages > MAX_STAGES) stages = MAX_STAGES;
+        if (stages < 1) stages = 1;
         while (split == 1 && stages * (A_BYTES + NP * 128) < NP * TILE * 4) ++stages;      // (the sums leave through them)
     }
     if (stages < 1 || stages > MAX_STAGES || few_smem(stages, NP, split) > most || (split == 1 && stages * (A_BYTES + NP * 128) < NP * TILE * 4))
@@ -517,6 +708,42 @@ static int many_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc,
                          stream, 1, mw, mx, ws, xs, o, T, N, kp, m_tiles, n_tiles, vec);
 }
 
+template <int SPLIT, int EPI>
+static int shared_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
+                          cudaStream_t stream) {
+    const int m_tiles = (T + 127) / 128, n_tiles = o.codes != nullptr ? padded(N / 2) / 64 : (N + 127) / 128;
+    const int cols = EPI == EPI_NONE ? N : N / 2, piece = o.dtype == JANIS_BF16 ? 8 : 4;
+    const int vec = cols % piece == 0 && ((uintptr_t)o.values & 15) == 0;
+    CUtensorMap mw, mx;
+    if (!make_map(&mw, WEIGHTS, wc, N, kp, 128) || !make_map(&mx, ROWS, xc, T, kp, 128))
+        return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
+    static std::once_flag once;
+    static cudaError_t e = cudaSuccess;
+    std::call_once(once, [] { e = cudaFuncSetAttribute(shared_rows_kernel<SPLIT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED_SMEM); });
+    if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
+    return launch_kernel("mx_product", shared_rows_kernel<SPLIT, EPI>, dim3(m_tiles * n_tiles * SPLIT), dim3(MANY_THREADS), SHARED_SMEM, stream, SPLIT,
+                         mw, mx, ws, xs, o, T, N, kp, m_tiles, vec);
+}
+
+template <int EPI>
+static int shared_rows_by(int split, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
+                          cudaStream_t stream) {
+    if (split > kp / BLOCK) return fail("mx_product: a split of %d is not possible here", split);
+    if (split == 2) return shared_rows_as<2, EPI>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (split == 4) return shared_rows_as<4, EPI>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if constexpr (EPI == EPI_NONE)
+        if (split == 8) return shared_rows_as<8, EPI>(xc, xs, wc, ws, o, T, N, kp, stream);
+    return fail("mx_product: a split of %d is not possible here", split);
+}
+
+static int shared_rows(int split, const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
+                       cudaStream_t stream) {
+    if (o.epi == EPI_NONE) return shared_rows_by<EPI_NONE>(split, xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_GELU) return shared_rows_by<EPI_GATED_GELU>(split, xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_SILU) return shared_rows_by<EPI_GATED_SILU>(split, xc, xs, wc, ws, o, T, N, kp, stream);
+    return shared_rows_by<EPI_GATED_CLAMP>(split, xc, xs, wc, ws, o, T, N, kp, stream);
+}
+
 template <int BN>
 static int many_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                      cudaStream_t stream) {
@@ -533,7 +760,8 @@ using namespace janis;
 
 static int g_kernel = 0;
 
-// Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 that of many with 256 and 128 rows of W a tile.  For tests and tuning.
+// Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 that of many with 256 and 128 rows of W a tile, 4 that of
+// many whose K is shared (by the CTAs of janis_mx_set_few).  For tests and tuning.
 JANIS_EXPORT void janis_mx_set_kernel(int kernel) { g_kernel = kernel; }
 
 static int g_split = 0, g_stages = 0;
@@ -559,6 +787,7 @@ JANIS_EXPORT int janis_mx_product(const uint8_t* xc, const uint8_t* xs, const ui
     const int kp = mx::padded(K);
     const int kernel = g_kernel != 0 ? g_kernel : T <= 64 ? 1 : 2;
     if (kernel == 1) return mx::few_rows(xc, xs, wc, ws, o, T, N, kp, g_split, g_stages, stream);
+    if (kernel == 4) return mx::shared_rows(g_split > 1 ? g_split : 2, xc, xs, wc, ws, o, T, N, kp, stream);
     return kernel == 2 ? mx::many_rows<256>(xc, xs, wc, ws, o, T, N, kp, stream) : mx::many_rows<128>(xc, xs, wc, ws, o, T, N, kp, stream);
 }
 

@@ -258,13 +258,12 @@ static int norm_rows(float* h, const TR* res, int n_part, size_t part_stride, co
                      float eps_next, const int* rows, uint8_t* codes, uint8_t* scales, int R, int H, cudaStream_t stream) {
     const bool vec = H % 8 == 0 && (((uintptr_t)h | (uintptr_t)res | (uintptr_t)w_post | (uintptr_t)w_next) & 15) == 0 && part_stride % 8 == 0;
     const int pieces = padded(H) / 8;
-    const int vpt = pieces <= 640 ? 1 : pieces <= 1280 ? 2 : 4;
-    if (!vec || pieces > 2560)
+    const int vpt = pieces <= 640 ? 1 : 2;
+    if (!vec || pieces > 1280)
         return launch_kernel("mx_norm_rows", norm_rows_kernel<TR>, dim3(R), dim3(256), 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post,
                              w_next, eps_next, rows, codes, scales, H);
     const dim3 block(((pieces + vpt - 1) / vpt + 31) / 32 * 32);
-    return launch_kernel("mx_norm_rows", vpt == 1 ? norm_rows_vec_kernel<TR, 1> : vpt == 2 ? norm_rows_vec_kernel<TR, 2> : norm_rows_vec_kernel<TR, 4>,
-                         dim3(R), block, 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
+    return launch_kernel("mx_norm_rows", vpt == 1 ? norm_rows_vec_kernel<TR, 1> : norm_rows_vec_kernel<TR, 2>, dim3(R), block, 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
 }
 
 static int blocks_for(size_t warps) {

@@ -349,6 +349,37 @@ def test_any_split_and_any_depth_of_the_ring(t, n, k):
 
 
 @GPU
+@pytest.mark.parametrize("kernel,split", [(1, 0), (2, 0), (3, 0), (4, 2), (4, 4), (4, 8)])
+@pytest.mark.parametrize("t,n,k", [(1, 144, 1024), (40, 1008, 1100), (129, 128, 2048), (260, 400, 1280)])
+def test_every_kernel_takes_every_size(t, n, k, kernel, split):
+    o = ops()
+    x, w = operands(t, n, k, seed=k)
+    want, tol = stands_for(x) @ stands_for(w).T, product_error(x, w)
+    try:
+        o.mx_set_kernel(kernel)
+        o.mx_set_few(split)
+        got = [o.linear_mx(x, w, torch.full((t, n), NAN, device="cuda")) for _ in range(2)]
+        assert torch.equal(*got), "the same call twice"
+        assert ((got[0].double() - want).abs() <= tol).all()
+        half = o.linear_mx(x, w, torch.empty(t, n, dtype=torch.bfloat16, device="cuda"))
+        assert torch.equal(half, got[0].bfloat16())
+        if n % 16 == 0 and split < 8:
+            for epi in (1, 3):
+                v = o.linear_mx(x, w, torch.full((t, n // 2), NAN, device="cuda"), epi)
+                rows, again = o.MxRows.empty(t, n // 2), o.MxRows.empty(t, n // 2)
+                rows.codes.fill_(5)
+                o.linear_mx(x, w, rows, epi)
+                o.mx_rows(v, again)
+                assert torch.equal(rows.codes, again.codes) and torch.equal(scale_rows(rows), scale_rows(again))
+                g, u = got[0].view(t, n // 16, 2, 8).unbind(2)
+                act = R._act(g.double().reshape(t, n // 2), 0 if epi == 1 else 1) * u.double().reshape(t, n // 2)
+                assert ((v.double() - act).abs() <= 2.0 ** -20 * act.abs() + 2.0 ** -22 * (g * u).abs().reshape(t, n // 2) + 1e-30).all()
+    finally:
+        o.mx_set_kernel()
+        o.mx_set_few()
+
+
+@GPU
 @pytest.mark.parametrize("t", [3, 40, 300])
 def test_groups_that_stand_for_nan_spoil_their_row_or_column(t):
     o = ops()
