@@ -128,20 +128,26 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         for (int i = 0; i < pre; ++i) load_x(rank + i * SPLIT, i);
         int filled = pre, s = 0;
         uint32_t phase = 0;
+        uint32_t free = 0;
         for (; filled < nk; ++filled) {
-            if (!mbar_wait(bar_empty + 8 * s, phase)) { atomicExch(&failed, 1); break; }
-            load_w(rank + filled * SPLIT, s);
-            load_x(rank + filled * SPLIT, s);
+            if (!free && !mbar_wait(bar_empty + 8 * s, phase)) { atomicExch(&failed, 1); break; }
+            const int now = s;
             if (++s == stages) { s = 0; phase ^= 1; }
+            free = mbar_peek(bar_empty + 8 * s, phase);
+            load_w(rank + filled * SPLIT, now);
+            load_x(rank + filled * SPLIT, now);
         }
         asked = filled;
     } else if (warp == 1 && elect_one()) {
         // ---- the thread that issues the products
         grid_dependency_wait();
-        int s = 0;
-        uint32_t phase = 0;
+        int next = 0;
+        uint32_t phase = 0, full = 0;
         for (int i = 0; i < nk; ++i) {
-            if (!mbar_wait(bar_full + 8 * s, phase)) { atomicExch(&failed, 1); break; }
+            const int s = next;
+            if (!full && !mbar_wait(bar_full + 8 * s, phase)) { atomicExch(&failed, 1); break; }
+            if (++next == stages) { next = 0; phase ^= 1; }
+            full = mbar_peek(bar_full + 8 * next, phase);
             fence_after_sync();
             const uint32_t a = stage0 + s * stage_bytes, b = a + A_BYTES, sc = scales0 + s * SCALE_BYTES;
             const uint32_t ta = tmem + NP + s * SCALE_COLS, tb = ta + 4;
@@ -151,7 +157,6 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             for (int g = 0; g < 4; ++g)                               // 32 bytes further along the swizzled row
                 umma_block(tmem, smem_desc(a + g * 32), smem_desc(b + g * 32), block_desc<WEIGHTS>(TILE, NP, g), ta, tb, (i > 0 || g > 0) ? 1u : 0u);
             umma_commit(bar_empty + 8 * s);                           // the stage is free once these have read it
-            if (++s == stages) { s = 0; phase ^= 1; }
         }
         umma_commit(bar_done);                                        // all products of this CTA have finished
     } else {
@@ -339,29 +344,36 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         grid_dependency_wait();
         for (int i = 0; i < pre; ++i) load_x(i, i, m);
         int filled = pre;
+        int s = pre == STAGES ? 0 : pre;
+        uint32_t phase = pre == STAGES ? 0 : 1, free = 0;             // (a stage that was never filled counts as free: parity 1 passes)
         bool ok = true;
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
             tile_at(i, m_tiles, n_tiles, m, n);
             for (int kb = i == blockIdx.x ? pre : 0; kb < blocks; ++kb, ++filled) {
-                const int s = filled % STAGES;
-                if (filled >= STAGES && !mbar_wait(bar_empty + 8 * s, (filled / STAGES - 1) & 1)) { atomicExch(&failed, 1); ok = false; break; }
-                load_w(s, kb, n * BN);
-                load_x(s, kb, m);
+                if (!free && !mbar_wait(bar_empty + 8 * s, phase)) { atomicExch(&failed, 1); ok = false; break; }
+                const int now = s;
+                if (++s == STAGES) { s = 0; phase ^= 1; }
+                free = mbar_peek(bar_empty + 8 * s, phase);
+                load_w(now, kb, n * BN);
+                load_x(now, kb, m);
             }
         }
         asked = filled;
     } else if (warp == 1 && elect_one()) {
         grid_dependency_wait();
-        int at = 0, turn = 0;
+        int next = 0, turn = 0;
+        uint32_t phase = 0, full = 0;
         bool ok = true;
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x, ++turn) {
             const int b = turn % BUFFERS;
             const uint32_t d = tmem + b * BN;
             if (turn >= BUFFERS && !mbar_wait(bar_drained + 8 * b, (turn / BUFFERS - 1) & 1)) { atomicExch(&failed, 1); break; }
             fence_after_sync();
-            for (int kb = 0; kb < blocks; ++kb, ++at) {
-                const int s = at % STAGES;
-                if (!mbar_wait(bar_full + 8 * s, (at / STAGES) & 1)) { atomicExch(&failed, 1); ok = false; break; }
+            for (int kb = 0; kb < blocks; ++kb) {
+                const int s = next;
+                if (!full && !mbar_wait(bar_full + 8 * s, phase)) { atomicExch(&failed, 1); ok = false; break; }
+                if (++next == STAGES) { next = 0; phase ^= 1; }
+                full = mbar_peek(bar_full + 8 * next, phase);
                 fence_after_sync();
                 const uint32_t x = stage0 + s * STAGE, w = x + X_BYTES, sc = scales0 + s * SCALE_BYTES;
                 const uint32_t tx = tmem + 256 + s * SCALE_COLS, tw = tx + 4;
@@ -452,14 +464,14 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 // ---------------------------------------------------------------------------
 // many rows of which there are not enough tiles for the SMs: a cluster shares K
 // ---------------------------------------------------------------------------
-constexpr int SHARED_STAGES = 4, SHARED_STAGE = X_BYTES + A_BYTES, SHARED_SCALES = 2 * BLOCK_BYTES;
-constexpr int SHARED_SMEM = SHARED_STAGES * (SHARED_STAGE + SHARED_SCALES) + 128 * 128 * 4 + 1024;
+constexpr int SHARED_STAGES = 5, SHARED_STAGE = X_BYTES + A_BYTES, SHARED_SCALES = 2 * BLOCK_BYTES;
+constexpr int shared_smem(int split) { return SHARED_STAGES * (SHARED_STAGE + SHARED_SCALES) + 128 * 128 * 4 / split * (split - 1) + 1024; }
 
-// where 16 bytes of sums (columns 4 c .. 4 c + 3 of row `row`) of a rank stand in the CTA that adds them up: the columns are turned by the row, so
-// that 32 rows that send the same columns do not meet in the same banks
+// where the sum for (row, column) stands among those that another CTA sent, or this one's own (place 0, over the idle stages): rows lie together,
+// since the 32 lanes that send have a row each
 template <int SPLIT>
-__device__ __forceinline__ uint32_t sums_at(int rank, int row, int c) {
-    return (uint32_t)((rank * (128 / SPLIT) + row) * 512 + ((c ^ (row & 31)) << 4));
+__device__ __forceinline__ int sums_at(int place, int row, int c) {
+    return (place * 128 + c) * (128 / SPLIT) + row;
 }
 
 template <int SPLIT, int EPI>
@@ -471,6 +483,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     __shared__ __align__(8) unsigned long long bars[2 * SHARED_STAGES + 2];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed, asked;
+    __shared__ float largest[EPI == EPI_NONE ? 1 : 256];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cg::this_cluster().block_rank(), tile = blockIdx.x / SPLIT, m = tile % m_tiles, n = tile / m_tiles;
     const int blocks = kp / BLOCK, nk = (blocks - rank + SPLIT - 1) / SPLIT;
@@ -484,7 +497,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         for (int i = 0; i < 2 * SHARED_STAGES + 2; ++i) mbar_init(bar_full + 8 * i, 1);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        mbar_expect_tx(bar_sums, SPLIT * mine * 512);
+        mbar_expect_tx(bar_sums, (SPLIT - 1) * mine * 512);
     }
     if (warp == 0) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), 256);
     fence_before_sync();
@@ -511,18 +524,22 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         grid_dependency_wait();
         for (int i = 0; i < pre; ++i) load_x(rank + i * SPLIT, i);
         int filled = pre;
+        uint32_t free = 0;
         for (; filled < nk; ++filled) {
-            const int s = filled % SHARED_STAGES;
-            if (!mbar_wait(bar_empty + 8 * s, (filled / SHARED_STAGES - 1) & 1)) { atomicExch(&failed, 1); break; }
+            const int s = filled % SHARED_STAGES, then = filled + 1;
+            if (!free && !mbar_wait(bar_empty + 8 * s, (filled / SHARED_STAGES - 1) & 1)) { atomicExch(&failed, 1); break; }
+            free = mbar_peek(bar_empty + 8 * (then % SHARED_STAGES), (then / SHARED_STAGES - 1) & 1);
             load_w(rank + filled * SPLIT, s);
             load_x(rank + filled * SPLIT, s);
         }
         asked = filled;
     } else if (warp == 1 && elect_one()) {
         grid_dependency_wait();
+        uint32_t full = 0;
         for (int i = 0; i < nk; ++i) {
             const int s = i % SHARED_STAGES;
-            if (!mbar_wait(bar_full + 8 * s, (i / SHARED_STAGES) & 1)) { atomicExch(&failed, 1); break; }
+            if (!full && !mbar_wait(bar_full + 8 * s, (i / SHARED_STAGES) & 1)) { atomicExch(&failed, 1); break; }
+            full = mbar_peek(bar_full + 8 * ((i + 1) % SHARED_STAGES), ((i + 1) / SHARED_STAGES) & 1);
             fence_after_sync();
             const uint32_t x = stage0 + s * SHARED_STAGE, w = x + X_BYTES, sc = scales0 + s * SHARED_SCALES, tx = tmem + 128 + s * 8, tw = tx + 4;
             scales_to_tmem(tx, sc);
@@ -545,6 +562,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             mbar_wait(bar_full + 8 * (j % SHARED_STAGES), (j / SHARED_STAGES) & 1);
     asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // everybody's barriers are there
 
+    float* own = reinterpret_cast<float*>(smem_raw + (stage0 - raw));
     if (warp >= 4) {
         const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane, owner = row / ROWS;
         uint32_t there, there_bar;
@@ -555,12 +573,15 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             uint32_t v[32];
             tmem_load32(v, tmem + ((uint32_t)(warp % 4 * 32) << 16) + half * 64 + c);
             tmem_wait_load();
-            if (row < rows) {
+            if (owner == rank) {
 #pragma unroll
-                for (int j = 0; j < 32; j += 4)
-                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];\n" ::"r"(
-                                     there + sums_at<SPLIT>(rank, row % ROWS, (half * 64 + c + j) / 4)),
-                                 "r"(v[j]), "r"(v[j + 1]), "r"(v[j + 2]), "r"(v[j + 3]), "r"(there_bar)
+                for (int j = 0; j < 32; ++j) own[sums_at<SPLIT>(0, row % ROWS, half * 64 + c + j)] = __uint_as_float(v[j]);
+            } else if (row < rows) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];\n" ::"r"(
+                                     there + 4 * (uint32_t)sums_at<SPLIT>(rank - (rank > owner), row % ROWS, half * 64 + c + j)),
+                                 "r"(v[j]), "r"(there_bar)
                                  : "memory");
             }
         }
@@ -579,22 +600,17 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         return;
     }
     if (warp < 4) return;
-    // ---- a run of one row's columns, added up in the order of the ranks
-    const int id = threadIdx.x - 128, row = id / (2 * SPLIT), c0 = id % (2 * SPLIT) * RUN, t = m * 128 + rank * ROWS + row;
+    // ---- a run of one row's columns, added up in the order of the ranks; a warp has 32 rows of the same run (or 16 of two)
+    const int id = threadIdx.x - 128, row = id % ROWS, run = id / ROWS, c0 = run * RUN, t = m * 128 + rank * ROWS + row;
     const bool live = row < mine;
+    const float* sums = reinterpret_cast<const float*>(smem_raw + (sums0 - raw));
     uint32_t v[RUN];
 #pragma unroll
-    for (int c = 0; c < RUN; c += 4) {
-        float f[4];
+    for (int c = 0; c < RUN; ++c) {
+        float f = 0.f;
 #pragma unroll
-        for (int r = 0; r < SPLIT; ++r) {
-            float g[4];
-            Vec16<float>::load(reinterpret_cast<const float*>(smem_raw + (sums0 - raw) + sums_at<SPLIT>(r, row, (c0 + c) / 4)), g);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = r == 0 ? g[e] : f[e] + g[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[c + e] = __float_as_uint(f[e]);
+        for (int r = 0; r < SPLIT; ++r) f += r == rank ? own[sums_at<SPLIT>(0, row, c0 + c)] : sums[sums_at<SPLIT>(r - (r > rank), row, c0 + c)];
+        v[c] = __float_as_uint(f);
     }
     if (EPI == EPI_NONE) {
         if (live) store_run<RUN>(v, o, (size_t)t * N + n * 128 + c0, N - n * 128 - c0, vec);
@@ -611,12 +627,14 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             if (live) store_run<RUN / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
             return;
         }
-        constexpr int HELD = RUN / 2;                                 // columns of a thread: 16 or 8 of a group of 32
+        constexpr int HELD = RUN / 2, RUNS = 32 / HELD;               // columns of a thread: 16 or 8 of a group of 32, the others in other warps
         float big = 0.f;
 #pragma unroll
         for (int j = 0; j < HELD; ++j) big = larger(big, __uint_as_float(v[j]));
+        largest[id] = big;
+        asm volatile("bar.sync 1, 256;\n" ::: "memory");
 #pragma unroll
-        for (int l = 1; l < 32 / HELD; l *= 2) big = larger(big, __shfl_xor_sync(0xffffffffu, big, l));
+        for (int j = 0; j < RUNS; ++j) big = larger(big, largest[(run / RUNS * RUNS + j) * ROWS + row]);
         const uint32_t byte = scale_byte_e4m3(big);
         const float inv = inverse_scale(byte);
         if (!live || c >= wide) return;
@@ -719,9 +737,9 @@ static int shared_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* w
         return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
     static std::once_flag once;
     static cudaError_t e = cudaSuccess;
-    std::call_once(once, [] { e = cudaFuncSetAttribute(shared_rows_kernel<SPLIT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED_SMEM); });
+    std::call_once(once, [] { e = cudaFuncSetAttribute(shared_rows_kernel<SPLIT, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_smem(SPLIT)); });
     if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
-    return launch_kernel("mx_product", shared_rows_kernel<SPLIT, EPI>, dim3(m_tiles * n_tiles * SPLIT), dim3(MANY_THREADS), SHARED_SMEM, stream, SPLIT,
+    return launch_kernel("mx_product", shared_rows_kernel<SPLIT, EPI>, dim3(m_tiles * n_tiles * SPLIT), dim3(MANY_THREADS), shared_smem(SPLIT), stream, SPLIT,
                          mw, mx, ws, xs, o, T, N, kp, m_tiles, vec);
 }
 
@@ -744,6 +762,55 @@ static int shared_rows(int split, const uint8_t* xc, const uint8_t* xs, const ui
     return shared_rows_by<EPI_GATED_CLAMP>(split, xc, xs, wc, ws, o, T, N, kp, stream);
 }
 
+// How many clusters of `split` CTAs of the kernel that shares K the GPU holds at once (a cluster lies within a GPC).
+template <int SPLIT>
+static int clusters_held() {
+    static int n = -1;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        cudaFuncSetAttribute(shared_rows_kernel<SPLIT, EPI_NONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, shared_smem(SPLIT));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(SPLIT * 16);
+        cfg.blockDim = dim3(MANY_THREADS);
+        cfg.dynamicSmemBytes = shared_smem(SPLIT);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = SPLIT;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, shared_rows_kernel<SPLIT, EPI_NONE>, &cfg) != cudaSuccess) {
+            n = 0;
+            cudaGetLastError();
+        }
+    });
+    return n;
+}
+
+// The kernel of a product: 1 few rows, 2 and 3 many with 256 and 128 rows of W a tile, 5, 6, 7 many whose K is shared by 2, 4, 8 CTAs.
+// Up to 64 rows the first, but where K is short (at 777, 1,000 weights and 32 rows 3.6 us against 3.1) or W alone fills the SMs (64 rows x 18,432 x
+// 2,304: 9.0 against 7.8).  Above, the least of what they take in us, as measured: a wave of tiles costs 0.22 a block of K and 1.2 at 128 rows of W,
+// 0.36 and 1.2 at 256, and 1.5 and 2.2 once; sharing costs 0.28 a block and 4.2, as long as all clusters are resident.
+static int choose(int T, int N, int blocks, const Out& o) {
+    const int sms = sm_count(), m_tiles = (T + 127) / 128;
+    const long long tiles128 = (long long)m_tiles * ((N + 127) / 128), tiles256 = (long long)m_tiles * ((N + 255) / 256);
+    if (T <= 16 || (T <= 64 && blocks > 8 && !(T > 48 && tiles128 * 8 >= sms * 7))) return 1;
+    const double cost128 = (tiles128 + sms - 1) / sms * (0.22 * blocks + 1.2) + 1.5, cost256 = (tiles256 + sms - 1) / sms * (0.36 * blocks + 1.2) + 2.2;
+    int best = cost128 <= cost256 ? 3 : 2;
+    double least = cost128 <= cost256 ? cost128 : cost256;
+    const int held[3] = {tiles128 <= sms / 2 ? clusters_held<2>() : 0, tiles128 <= sms / 4 ? clusters_held<4>() : 0,
+                         tiles128 <= sms / 8 && o.epi == EPI_NONE ? clusters_held<8>() : 0};
+    for (int i = 0; i < 3; ++i) {
+        const int split = 2 << i;
+        const double cost = 0.28 * ((blocks + split - 1) / split) + 4.2;
+        if (tiles128 <= held[i] && blocks >= 2 * split && cost < least) {
+            best = 5 + i;
+            least = cost;
+        }
+    }
+    return best;
+}
+
 template <int BN>
 static int many_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                      cudaStream_t stream) {
@@ -761,7 +828,7 @@ using namespace janis;
 static int g_kernel = 0;
 
 // Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 that of many with 256 and 128 rows of W a tile, 4 that of
-// many whose K is shared (by the CTAs of janis_mx_set_few).  For tests and tuning.
+// many whose K is shared (by the CTAs of janis_mx_set_few), 5, 6 and 7 the same by 2, 4 and 8.  For tests and tuning.
 JANIS_EXPORT void janis_mx_set_kernel(int kernel) { g_kernel = kernel; }
 
 static int g_split = 0, g_stages = 0;
@@ -785,8 +852,9 @@ JANIS_EXPORT int janis_mx_product(const uint8_t* xc, const uint8_t* xs, const ui
     if (K > 1 << 30) return fail("mx_product: a row has at most 2^30 values, found %d", K);
     const mx::Out o = {out, out_codes, out_scales, out_dtype, epi, limit, alpha, up_add};
     const int kp = mx::padded(K);
-    const int kernel = g_kernel != 0 ? g_kernel : T <= 64 ? 1 : 2;
+    const int kernel = g_kernel != 0 ? g_kernel : mx::choose(T, N, kp / mx::BLOCK, o);
     if (kernel == 1) return mx::few_rows(xc, xs, wc, ws, o, T, N, kp, g_split, g_stages, stream);
+    if (kernel >= 5) return mx::shared_rows(1 << (kernel - 4), xc, xs, wc, ws, o, T, N, kp, stream);
     if (kernel == 4) return mx::shared_rows(g_split > 1 ? g_split : 2, xc, xs, wc, ws, o, T, N, kp, stream);
     return kernel == 2 ? mx::many_rows<256>(xc, xs, wc, ws, o, T, N, kp, stream) : mx::many_rows<128>(xc, xs, wc, ws, o, T, N, kp, stream);
 }

@@ -40,6 +40,16 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t smem) {
     d |= (uint64_t)1 << 46;
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(d) : "memory");
 }
+// Whether a phase has ended, asked ahead of need: the answer takes some 170 clocks, which the copies or products that are issued meanwhile hide
+// (a product of 128 x 128 x 32 takes 64).  The rest of the wait, where there is one, is mbar_wait's.
+__device__ __forceinline__ uint32_t mbar_peek(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done;
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes),
                  "r"(bar)
