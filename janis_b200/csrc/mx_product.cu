@@ -20,6 +20,7 @@
 // Every wait is bounded: a CTA that gives up counts it (janis_mx_timeouts_async), waits for its copies, frees its tensor memory
 // and leaves without a result.  No load here uses cluster multicast.
 #include <cooperative_groups.h>
+#include <limits.h>
 
 #include "mx_tc05.cuh"
 
@@ -840,9 +841,26 @@ JANIS_EXPORT void janis_mx_set_few(int split, int stages) {
 }
 
 // x: codes [T, padded K], W: codes [N, padded K / 2]; out [T, N] (N / 2 with a gated epilogue) of out_dtype, or 8-bit rows
-JANIS_EXPORT int janis_mx_product(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, void* out, int out_dtype,
-                                  uint8_t* out_codes, uint8_t* out_scales, int T, int N, int K, int epi, float limit, float alpha,
-                                  float up_add, cudaStream_t stream) {
+// The arguments come as one block of 8-byte fields.
+struct ProductArgs {
+    const uint8_t *xc, *xs, *wc, *ws;
+    void* out;
+    long long out_dtype;
+    uint8_t *out_codes, *out_scales;
+    long long T, N, K, epi;
+    double limit, alpha, up_add;
+    cudaStream_t stream;
+};
+JANIS_EXPORT int janis_mx_product(const void* block) {
+    ProductArgs a;
+    memcpy(&a, block, sizeof(a));
+    const uint8_t *xc = a.xc, *xs = a.xs, *wc = a.wc, *ws = a.ws;
+    void* out = a.out;
+    uint8_t *out_codes = a.out_codes, *out_scales = a.out_scales;
+    if (a.T > INT_MAX || a.N > INT_MAX || a.K > INT_MAX) return fail("mx_product: sizes pass 2^31");
+    const int out_dtype = (int)a.out_dtype, T = (int)a.T, N = (int)a.N, K = (int)a.K, epi = (int)a.epi;
+    const float limit = (float)a.limit, alpha = (float)a.alpha, up_add = (float)a.up_add;
+    cudaStream_t stream = a.stream;
     if (T <= 0 || N <= 0) return 0;
     if (K <= 0) return fail("mx_product: a row has no values");
     if (epi != mx::EPI_NONE && epi != mx::EPI_GATED_GELU && epi != mx::EPI_GATED_SILU && epi != mx::EPI_GATED_CLAMP)

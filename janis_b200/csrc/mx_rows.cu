@@ -1,5 +1,7 @@
 // Rows in and out of the 8-bit microscaling form (mx.cuh): the norms and the gated activation that leave it for the products
 // behind them, plain rows, the weights' 4-bit form at load, and the values that either form stands for.
+#include <limits.h>
+
 #include "mx.cuh"
 
 namespace janis {
@@ -82,46 +84,49 @@ __device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* co
     if ((threadIdx.x & 15) == 0) *reinterpret_cast<uint32_t*>(scales + scale_at(r, j / 16, blocks)) = four;
 }
 
-// The same with the row in registers: thread i takes the pieces of 8 values i, i + blockDim, ... (H a multiple of 8, at most VPT of them a
-// thread), so that each input is read once, 16 bytes at a time, and a row's scales leave four at a time.
+// eight values of the residual as they are stored
+template <typename T> struct Eight;
+template <> struct Eight<bf16> {
+    uint4 raw;
+    __device__ __forceinline__ void load(const bf16* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ float get(int e) const {               // (e is a constant where this is used)
+        const uint32_t w = e / 2 == 0 ? raw.x : e / 2 == 1 ? raw.y : e / 2 == 2 ? raw.z : raw.w;
+        return __uint_as_float(e % 2 ? w & 0xffff0000u : w << 16);
+    }
+};
+template <> struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) { load_eight(p, v); }
+    __device__ __forceinline__ float get(int e) const { return v[e]; }
+};
+
+// The same with the row in registers: thread i takes the pieces of 8 values i, i + blockDim, ... (H a multiple of 8, at most VPT of them), so that
+// each input is read once, 16 bytes at a time, and a row's scales leave four at a time.  Bound by memory at many rows, where what counts is how
+// many rows an SM has on its way: the residual stays as it is stored, the norms' weights are read where they are used, and a thread takes two
+// pieces.  8,192 rows of 2,304: 43.2 us with one piece a thread, 37.9 with two, 40.3 with five, 59.8 with nine (a warp a row); 31.9 at the copy's
+// bandwidth.  Held weights and eight floats of the residual a thread: 60.0; rows that the copy engine brings into a ring: 66.7.  At few rows,
+// bound by latency, one piece: one row 2.4 us, with two 2.8.
 template <typename TR, int VPT>
 __global__ void __launch_bounds__(640)
-norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_part, size_t part_stride, const float* __restrict__ w_post,
-                     float eps_post, const float* __restrict__ w_next, float eps_next, const int* __restrict__ rows,
-                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int H) {
+norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, const float* __restrict__ w_post, float eps_post,
+                      const float* __restrict__ w_next, float eps_next, const int* __restrict__ rows, uint8_t* __restrict__ codes,
+                      uint8_t* __restrict__ scales, int H) {
     __shared__ float scratch[32];
     const int r = blockIdx.x, pieces = H / 8, all = padded(H) / 8;
     grid_dependents_launch();
-    float wn[VPT][8], wp[VPT][8];
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) {                                   // (the norms' weights are constants of the model)
-        const int j = threadIdx.x + k * blockDim.x;
-        if (j < pieces) {
-            load_eight(w_next + j * 8, wn[k]);
-            if (w_post != nullptr) load_eight(w_post + j * 8, wp[k]);
-        }
-    }
     grid_dependency_wait();
     float* hr = h + (size_t)(rows ? rows[r] : r) * H;
-    float v[VPT][8], hv[VPT][8];
+    Eight<TR> v[VPT];
+    float hv[VPT][8];
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int j = threadIdx.x + k * blockDim.x;
         if (j < pieces) {
+            if (res != nullptr) v[k].load(res + (size_t)r * H + j * 8);
             load_eight(hr + j * 8, hv[k]);
-            if (res != nullptr) {
-                const TR* rr = res + (size_t)r * H + j * 8;
-                load_eight(rr, v[k]);
-                for (int p = 1; p < n_part; ++p) {
-                    float more[8];
-                    load_eight(rr + p * part_stride, more);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[k][e] += more[e];
-                }
-            }
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[k][e] = hv[k][e] = wn[k][e] = wp[k][e] = 0.f;
+            for (int e = 0; e < 8; ++e) hv[k][e] = 0.f;
         }
     }
     float ss = 0.f;
@@ -130,8 +135,9 @@ norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_pa
         if (w_post != nullptr) {
 #pragma unroll
             for (int k = 0; k < VPT; ++k)
+                if ((int)threadIdx.x + k * (int)blockDim.x < pieces)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(v[k][e], v[k][e], ss);
+                    for (int e = 0; e < 8; ++e) ss = fmaf(v[k].get(e), v[k].get(e), ss);
             ss = block_sum(ss, scratch);
             inv = 1.0f / sqrtf(ss / (float)H + eps_post);
             ss = 0.f;
@@ -139,9 +145,17 @@ norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_pa
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int j = threadIdx.x + k * blockDim.x;
+            if (j >= pieces) continue;
+            if (w_post != nullptr) {
+                float w[8];
+                load_eight(w_post + j * 8, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) hv[k][e] += w_post != nullptr ? v[k][e] * inv * wp[k][e] : v[k][e];
-            if (j < pieces) store_eight(hr + j * 8, hv[k]);
+                for (int e = 0; e < 8; ++e) hv[k][e] += v[k].get(e) * inv * w[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) hv[k][e] += v[k].get(e);
+            }
+            store_eight(hr + j * 8, hv[k]);
         }
     }
 #pragma unroll
@@ -154,8 +168,12 @@ norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_pa
     for (int k = 0; k < VPT; ++k) {
         const int j = threadIdx.x + k * blockDim.x;
         if (j - (int)(threadIdx.x & 31) >= all) break;                // (a whole warp)
+        float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) hv[k][e] = j < pieces ? hv[k][e] * inv * wn[k][e] : 0.f;
+        for (int e = 0; e < 8; ++e) w[e] = 0.f;
+        if (j < pieces) load_eight(w_next + j * 8, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hv[k][e] = hv[k][e] * inv * w[e];
         store_eight_of_group(hv[k], codes, scales, r, j, all / 16, j < all);
     }
 }
@@ -258,12 +276,13 @@ static int norm_rows(float* h, const TR* res, int n_part, size_t part_stride, co
                      float eps_next, const int* rows, uint8_t* codes, uint8_t* scales, int R, int H, cudaStream_t stream) {
     const bool vec = H % 8 == 0 && (((uintptr_t)h | (uintptr_t)res | (uintptr_t)w_post | (uintptr_t)w_next) & 15) == 0 && part_stride % 8 == 0;
     const int pieces = padded(H) / 8;
-    const int vpt = pieces <= 640 ? 1 : 2;
-    if (!vec || pieces > 1280)
+    if (!vec || n_part > 1 || pieces > 1920)
         return launch_kernel("mx_norm_rows", norm_rows_kernel<TR>, dim3(R), dim3(256), 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post,
                              w_next, eps_next, rows, codes, scales, H);
-    const dim3 block(((pieces + vpt - 1) / vpt + 31) / 32 * 32);
-    return launch_kernel("mx_norm_rows", vpt == 1 ? norm_rows_vec_kernel<TR, 1> : norm_rows_vec_kernel<TR, 2>, dim3(R), block, 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
+    const int vpt = pieces > 1280 ? 3 : pieces > 640 || (R >= 768 && pieces > 160) ? 2 : 1;
+    const auto kernel = vpt == 1 ? norm_rows_vec_kernel<TR, 1> : vpt == 2 ? norm_rows_vec_kernel<TR, 2> : norm_rows_vec_kernel<TR, 3>;
+    return launch_kernel("mx_norm_rows", kernel, dim3(R), dim3(((pieces + vpt - 1) / vpt + 31) / 32 * 32), 0, stream, 1, h, res, w_post, eps_post,
+                         w_next, eps_next, rows, codes, scales, H);
 }
 
 static int blocks_for(size_t warps) {
@@ -292,9 +311,33 @@ JANIS_EXPORT const char* janis_last_error() { return error_buffer(); }
 JANIS_EXPORT void janis_mx_set_overlap(int on) { overlap_launches() = on; }
 
 // h [R or more, H] float; res [n_part, R, H] or null; rows [R] or null (with res: null); codes [R, padded H]
-JANIS_EXPORT int janis_mx_norm_rows(float* h, const void* res, int res_dtype, int n_part, long long part_stride, const float* w_post,
-                                    float eps_post, const float* w_next, float eps_next, const int* rows, uint8_t* codes,
-                                    uint8_t* scales, int R, int H, cudaStream_t stream) {
+// The arguments come as one block of 8-byte fields.
+struct NormArgs {
+    float* h;
+    const void* res;
+    long long res_dtype, n_part, part_stride;
+    const float* w_post;
+    double eps_post;
+    const float* w_next;
+    double eps_next;
+    const int* rows;
+    uint8_t *codes, *scales;
+    long long R, H;
+    cudaStream_t stream;
+};
+JANIS_EXPORT int janis_mx_norm_rows(const void* block) {
+    NormArgs a;
+    memcpy(&a, block, sizeof(a));
+    float* h = a.h;
+    const void* res = a.res;
+    const float *w_post = a.w_post, *w_next = a.w_next;
+    const float eps_post = (float)a.eps_post, eps_next = (float)a.eps_next;
+    const int* rows = a.rows;
+    uint8_t *codes = a.codes, *scales = a.scales;
+    if (a.R > INT_MAX || a.H > INT_MAX) return fail("mx_norm_rows: sizes pass 2^31");
+    const int res_dtype = (int)a.res_dtype, n_part = (int)a.n_part, R = (int)a.R, H = (int)a.H;
+    const long long part_stride = a.part_stride;
+    cudaStream_t stream = a.stream;
     if (R <= 0) return 0;
     if (H <= 0) return fail("mx_norm_rows: a row has no values");
     if (res != nullptr && rows != nullptr) return fail("mx_norm_rows: rows are gathered without a residual only");

@@ -211,11 +211,11 @@ def low_bits():
         _need_cuda()
         lib = build.low_bits_library()
         P, I, F = c_void_p, c_int, c_float
-        lib.janis_mx_norm_rows.argtypes = [P, P, I, I, c_longlong, P, F, P, F, P, P, P, I, I, P]
+        lib.janis_mx_norm_rows.argtypes = [ctypes.c_char_p]
         lib.janis_mx_rows.argtypes = [P, I, I, F, F, F, P, P, I, I, P]
         lib.janis_mx_weight.argtypes = [P, I, P, P, I, I, P]
         lib.janis_mx_values.argtypes = [P, P, I, P, I, I, I, P]
-        lib.janis_mx_product.argtypes = [P, P, P, P, P, I, P, P, I, I, I, I, F, F, F, P]
+        lib.janis_mx_product.argtypes = [ctypes.c_char_p]
         lib.janis_mx_set_few.argtypes = [I, I]
         lib.janis_mx_set_few.restype = None
         lib.janis_mx_set_kernel.argtypes = [I]
