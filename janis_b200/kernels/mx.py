@@ -29,7 +29,7 @@ def _padded(k: int) -> int:
     return (k + BLOCK - 1) // BLOCK * BLOCK
 
 
-_U8 = torch.uint8
+_U8, _F32 = torch.uint8, torch.float32
 
 
 class _Mx:
@@ -131,8 +131,19 @@ def mx_weight(w) -> MxWeight:
 
 def norm_to_rows(h, res, w_post, eps_post, w_next, eps_next, out: MxRows, n_part: int = 1, rows=None) -> MxRows:
     """`rmsnorm` (res None) and `add_rmsnorm` with 8-bit rows as their output."""
-    H = h.shape[1]
-    R = out.rows if res is None else h.shape[0]
+    lib = _ops._low_bits or _ops.low_bits()
+    shape, wide = h.shape, (out.width,)
+    # what a decode step calls, checked at once; whatever is not this is looked at one by one below
+    if (res is not None and w_next is not None and n_part == 1 and rows is None and shape == (out.rows, out.width) == res.shape
+            and (w_post is None or (w_post.dtype is _F32 and w_post.shape == wide and w_post.is_contiguous() and w_post.is_cuda))
+            and w_next.dtype is _F32 and w_next.shape == wide and w_next.is_contiguous() and w_next.is_cuda
+            and h.dtype is _F32 and h.is_contiguous() and h.is_cuda and res.is_contiguous() and res.is_cuda and res.dtype in _ops._DT):
+        _ops._check(lib, lib.janis_mx_norm_rows(_NORM(
+            h.data_ptr(), res.data_ptr(), _ops._DT[res.dtype], 1, 0, w_post.data_ptr() if w_post is not None else 0, eps_post,
+            w_next.data_ptr(), eps_next, 0, out.codes.data_ptr(), out.scales.data_ptr(), out.rows, out.width, _ops._stream())))
+        return out
+    H = shape[1]
+    R = out.rows if res is None else shape[0]
     if w_next is None:
         raise _ops.KernelError("add_rmsnorm: 8-bit rows are the second norm's output, which has no weight here")
     t = _ops._t
@@ -142,7 +153,6 @@ def norm_to_rows(h, res, w_post, eps_post, w_next, eps_next, out: MxRows, n_part
         p_res, dt, stride = 0, 0, 0
     else:
         p_res, dt, stride = t(res, "res", _ops._FLOATS, (R, H) if n_part == 1 else (n_part, R, H)), _ops._DT[res.dtype], R * H
-    lib = _ops._low_bits or _ops.low_bits()
     block = _NORM(t(h, "h", torch.float32, (None, H)), p_res, dt, n_part, stride,
                   t(w_post, "w_post", torch.float32, (H,)) if w_post is not None else 0, eps_post,
                   t(w_next, "w_next", torch.float32, (H,)), eps_next, t(rows, "rows", torch.int32, (R,)) if rows is not None else 0,
