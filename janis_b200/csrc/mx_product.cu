@@ -62,6 +62,65 @@ constexpr int few_smem(int stages, int NP, int split) {
     return stages * (A_BYTES + NP * 128 + SCALE_BYTES) + 1024 + (split > 1 ? NP * TILE * 4 : 0);
 }
 
+// The end of a tile of few rows: sums [SPLIT][rows][128 / SPLIT] of rows of W from row0 on, by 128 threads.
+template <int SPLIT>
+__device__ __forceinline__ void store_rows(const float* sums, int rows, int t0, int row0, int id, int N, const Out& o) {
+    constexpr int SHARE = TILE / SPLIT;
+    const auto sum_at = [&](int m, int row) {                         // in the order of the ranks
+        float v = sums[m * SHARE + row];
+#pragma unroll
+        for (int r = 1; r < SPLIT; ++r) v += sums[(r * rows + m) * SHARE + row];
+        return v;
+    };
+    if (o.epi == EPI_NONE) {
+        const int row = id % SHARE, n = row0 + row;
+        if (n >= N) return;
+        for (int m = id / SHARE; m < rows; m += SPLIT) {
+            const float v = sum_at(m, row);
+            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * N + n] = from_float<bf16>(v);
+            else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * N + n] = v;
+        }
+        return;
+    }
+    // a gate's up stands 8 rows behind it; for 8-bit rows a warp has the 32 columns of a group (SHARE is 64 at least)
+    constexpr int COLS = SHARE / 2;
+    const int j = id % COLS, c = row0 / 2 + j, row = j / 8 * 16 + j % 8;
+    const int all = N / 2, wide = o.codes != nullptr ? padded(all) : all;
+    if (c >= wide) return;                                            // (for 8-bit rows a whole warp)
+    constexpr int AT_ONCE = 4, STEP = 128 / COLS;                     // rows of x whose latencies (two loads, an exponential, a quotient, shuffles) overlap
+    for (int m0 = id / COLS; m0 < rows; m0 += AT_ONCE * STEP) {
+        float v[AT_ONCE], big[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int m = m0 + u * STEP;
+            v[u] = c < all && m < rows ? gated(sum_at(m, row), sum_at(m, row + 8), o.epi, o) : 0.f;
+            big[u] = fabsf(v[u]);
+        }
+        if (o.codes == nullptr) {
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int m = m0 + u * STEP;
+                if (m >= rows) break;
+                if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * all + c] = from_float<bf16>(v[u]);
+                else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * all + c] = v[u];
+            }
+            continue;
+        }
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1)
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) big[u] = larger(big[u], __shfl_xor_sync(0xffffffffu, big[u], s));
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            const int m = m0 + u * STEP;
+            if (m >= rows) break;
+            const uint32_t byte = scale_byte_e4m3(big[u]);
+            o.codes[(size_t)(t0 + m) * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v[u] * inverse_scale(byte), 0.f);
+            if ((id & 31) == 0) o.scales[scale_at(t0 + m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
+        }
+    }
+}
+
 template <int SPLIT>
 __global__ void __launch_bounds__(128)
 few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
@@ -206,42 +265,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
         return;
     }
-    const auto sum_at = [&](int m, int row) {                         // in the order of the ranks
-        float v = sums[m * SHARE + row];
-#pragma unroll
-        for (int r = 1; r < SPLIT; ++r) v += sums[(r * rows + m) * SHARE + row];
-        return v;
-    };
-    const int row0 = n0 + rank * SHARE;
-    if (o.epi == EPI_NONE) {
-        const int row = threadIdx.x % SHARE, n = row0 + row;
-        if (n >= N) return;
-        for (int m = threadIdx.x / SHARE; m < rows; m += SPLIT) {
-            const float v = sum_at(m, row);
-            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * N + n] = from_float<bf16>(v);
-            else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * N + n] = v;
-        }
-        return;
-    }
-    // a gate's up stands 8 rows behind it; for 8-bit rows a warp has the 32 columns of a group (SHARE is 64 at least)
-    constexpr int COLS = SHARE / 2;
-    const int j = threadIdx.x % COLS, c = row0 / 2 + j, row = j / 8 * 16 + j % 8;
-    const int all = N / 2, wide = o.codes != nullptr ? padded(all) : all;
-    if (c >= wide) return;                                            // (for 8-bit rows a whole warp)
-    for (int m = threadIdx.x / COLS; m < rows; m += 128 / COLS) {
-        const float v = c < all ? gated(sum_at(m, row), sum_at(m, row + 8), o.epi, o) : 0.f;
-        if (o.codes != nullptr) {
-            float big = fabsf(v);
-#pragma unroll
-            for (int s = 16; s > 0; s >>= 1) big = larger(big, __shfl_xor_sync(0xffffffffu, big, s));
-            const uint32_t byte = scale_byte_e4m3(big);
-            o.codes[(size_t)(t0 + m) * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v * inverse_scale(byte), 0.f);
-            if (lane == 0) o.scales[scale_at(t0 + m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
-        } else if (c < all) {
-            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * all + c] = from_float<bf16>(v);
-            else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * all + c] = v;
-        }
-    }
+    store_rows<SPLIT>(sums, rows, t0, n0 + rank * SHARE, threadIdx.x, N, o);
 }
 
 // ---------------------------------------------------------------------------
@@ -789,13 +813,14 @@ static int clusters_held() {
 }
 
 // The kernel of a product: 1 few rows, 2 and 3 many with 256 and 128 rows of W a tile, 5, 6, 7 many whose K is shared by 2, 4, 8 CTAs.
-// Up to 64 rows the first, but where K is short (at 777, 1,000 weights and 32 rows 3.6 us against 3.1) or W alone fills the SMs (64 rows x 18,432 x
+// Up to 64 rows the first (32 with a gated epilogue, which is the longer the more rows a thread has: 64 rows x 28,672 x 3,584 27.5 us against 17.4),
+// but where K is short (at 777, 1,000 weights and 32 rows 3.6 us against 3.1) or W alone fills the SMs (64 rows x 18,432 x
 // 2,304: 9.0 against 7.8).  Above, the least of what they take in us, as measured: a wave of tiles costs 0.22 a block of K and 1.2 at 128 rows of W,
 // 0.36 and 1.2 at 256, and 1.5 and 2.2 once; sharing costs 0.28 a block and 4.2, as long as all clusters are resident.
 static int choose(int T, int N, int blocks, const Out& o) {
     const int sms = sm_count(), m_tiles = (T + 127) / 128;
     const long long tiles128 = (long long)m_tiles * ((N + 127) / 128), tiles256 = (long long)m_tiles * ((N + 255) / 256);
-    if (T <= 16 || (T <= 64 && blocks > 8 && !(T > 48 && tiles128 * 8 >= sms * 7))) return 1;
+    if (T <= 16 || (T <= (o.epi == EPI_NONE ? 64 : 32) && blocks > 8 && !(T > 48 && tiles128 * 8 >= sms * 7))) return 1;
     const double cost128 = (tiles128 + sms - 1) / sms * (0.22 * blocks + 1.2) + 1.5, cost256 = (tiles256 + sms - 1) / sms * (0.36 * blocks + 1.2) + 2.2;
     int best = cost128 <= cost256 ? 3 : 2;
     double least = cost128 <= cost256 ? cost128 : cost256;
