@@ -317,6 +317,49 @@ __device__ __forceinline__ void store_run(const uint32_t* v, const Out& o, size_
     }
 }
 
+// The end of a row's run of COLS columns of sums from column n0 on (rows of W), by the thread that holds them.
+template <int COLS, int EPI>
+__device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, int t, int n0, int T, int N, bool vec) {
+    if (t >= T) return;
+    if constexpr (EPI == EPI_NONE) {
+        store_run<COLS>(v, o, (size_t)t * N + n0, N - n0, vec);
+    } else {
+        const int cols = N / 2, wide = o.codes != nullptr ? padded(cols) : cols, c = n0 / 2;
+#pragma unroll
+        for (int u = 0; u < COLS / 16; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[u * 8 + j] = __float_as_uint(gated(__uint_as_float(v[u * 16 + j]), __uint_as_float(v[u * 16 + 8 + j]), EPI, o));
+        if (o.codes == nullptr) {
+            store_run<COLS / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
+            return;
+        }
+#pragma unroll
+        for (int g = 0; g < COLS / 64; ++g) {                         // (columns past the end are products with zeros)
+            float big = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) big = larger(big, __uint_as_float(v[g * 32 + j]));
+            const uint32_t byte = scale_byte_e4m3(big);
+            const float inv = inverse_scale(byte);
+            uint32_t q[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t* p = v + g * 32 + j * 4;
+                q[j] = byte == 255u ? 0u
+                                    : two_e4m3(__uint_as_float(p[0]) * inv, __uint_as_float(p[1]) * inv) |
+                                          two_e4m3(__uint_as_float(p[2]) * inv, __uint_as_float(p[3]) * inv) << 16;
+            }
+            const int cg = c + g * 32;
+            if (cg < wide) {
+                uint4* to = reinterpret_cast<uint4*>(o.codes + (size_t)t * wide + cg);
+                to[0] = make_uint4(q[0], q[1], q[2], q[3]);
+                to[1] = make_uint4(q[4], q[5], q[6], q[7]);
+                o.scales[scale_at(t, cg / BLOCK, wide / BLOCK) + cg % BLOCK / GROUP] = (uint8_t)byte;
+            }
+        }
+    }
+}
+
 template <int BN, int EPI>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
@@ -416,7 +459,6 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     } else if (warp >= 4) {
         grid_dependency_wait();
         const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane;  // (a warp reaches the quarter of tensor memory that its number says)
-        const int cols = EPI == EPI_NONE ? N : N / 2, wide = o.codes != nullptr ? padded(cols) : cols;
         int turn = 0;
         for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++turn) {
             const int b = turn % BUFFERS;
@@ -432,46 +474,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
             fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_drained + 8 * b);
-            const int t = m * 128 + row;
-            if (t >= T) continue;
-            if (EPI == EPI_NONE) {
-                const int c = n * BN + half * COLS;
-                store_run<COLS>(v, o, (size_t)t * N + c, N - c, vec);
-                continue;
-            }
-            const int c = (n * BN + half * COLS) / 2;
-#pragma unroll
-            for (int u = 0; u < COLS / 16; ++u)
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    v[u * 8 + j] = __float_as_uint(gated(__uint_as_float(v[u * 16 + j]), __uint_as_float(v[u * 16 + 8 + j]), EPI, o));
-            if (o.codes == nullptr) {
-                store_run<COLS / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
-                continue;
-            }
-#pragma unroll
-            for (int g = 0; g < COLS / 64; ++g) {                     // (columns past the end are products with zeros)
-                float big = 0.f;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) big = larger(big, __uint_as_float(v[g * 32 + j]));
-                const uint32_t byte = scale_byte_e4m3(big);
-                const float inv = inverse_scale(byte);
-                uint32_t q[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t* p = v + g * 32 + j * 4;
-                    q[j] = byte == 255u ? 0u
-                                        : two_e4m3(__uint_as_float(p[0]) * inv, __uint_as_float(p[1]) * inv) |
-                                              two_e4m3(__uint_as_float(p[2]) * inv, __uint_as_float(p[3]) * inv) << 16;
-                }
-                const int cg = c + g * 32;
-                if (cg < wide) {
-                    uint4* to = reinterpret_cast<uint4*>(o.codes + (size_t)t * wide + cg);
-                    to[0] = make_uint4(q[0], q[1], q[2], q[3]);
-                    to[1] = make_uint4(q[4], q[5], q[6], q[7]);
-                    o.scales[scale_at(t, cg / BLOCK, wide / BLOCK) + cg % BLOCK / GROUP] = (uint8_t)byte;
-                }
-            }
+            finish_run<COLS, EPI>(v, o, m * 128 + row, n * BN + half * COLS, T, N, vec);
         }
     } else {
         grid_dependency_wait();
@@ -484,6 +487,138 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         for (int j = asked > STAGES ? asked - STAGES : 0; j < asked; ++j) mbar_wait(bar_full + 8 * (j % STAGES), (j / STAGES) & 1);
     }
     if (warp == 0) tmem_free(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------
+// many rows, two CTAs as one
+// ---------------------------------------------------------------------------
+constexpr int PAIR_STAGES = 6, PAIR_STAGE = X_BYTES + A_BYTES;
+constexpr int PAIR_SMEM = PAIR_STAGES * (PAIR_STAGE + SCALE_BYTES) + 1024;
+
+// 256 rows of x by 256 of W: each SM holds half of both, so that it fetches and reads two thirds of what a tile of 128 x 256 wants for the same
+// products, and its sums are 128 rows of 256 columns as there.
+template <int EPI>
+__global__ void __launch_bounds__(MANY_THREADS, 1)
+pair_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_ws,
+                 const __grid_constant__ CUtensorMap map_xs, const Out o, int T, int N, int kp, int m_tiles, int n_tiles, int vec) {
+    constexpr int COLS = 128;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) unsigned long long bars[2 * PAIR_STAGES + 2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cg::this_cluster().block_rank();
+    const int blocks = kp / BLOCK, tiles = m_tiles * n_tiles, first = blockIdx.x / 2, step = gridDim.x / 2;
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
+    const uint32_t stage0 = (raw + 1023) & ~1023u, scales0 = stage0 + PAIR_STAGES * PAIR_STAGE;
+    const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
+    const uint32_t bar_empty = bar_full + 8 * PAIR_STAGES, bar_sums = bar_full + 16 * PAIR_STAGES, bar_drained = bar_sums + 8;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2 * PAIR_STAGES + 1; ++i) mbar_init(bar_full + 8 * i, 1);
+        mbar_init(bar_drained, 16);                                   // the draining warps of both
+        failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 0) pair_tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), 512);
+    fence_before_sync();
+    __syncthreads();
+    cg::this_cluster().sync();                                        // the barriers of both are there
+    fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    grid_dependents_launch();
+
+    if (warp == 0 && elect_one()) {
+        // ---- the copies of this CTA's half, counted in by the first CTA's barriers
+        const uint32_t full = in_cta(bar_full, 0);
+        const auto load_w = [&](int s, int kb, int n) {
+            if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * (X_BYTES + A_PACKED + 3 * BLOCK_BYTES));
+            pair_load_2d(stage0 + s * PAIR_STAGE + X_BYTES, &map_w, kb * BLOCK, n * 256 + (int)rank * 128, full + 8 * s);
+            pair_load_3d(scales0 + s * SCALE_BYTES + BLOCK_BYTES, &map_ws, 0, kb * 2, n * 2, full + 8 * s);
+        };
+        const auto load_x = [&](int s, int kb, int m) {
+            pair_load_2d(stage0 + s * PAIR_STAGE, &map_x, kb * BLOCK, m * 256 + (int)rank * 128, full + 8 * s);
+            pair_load_3d(scales0 + s * SCALE_BYTES, &map_xs, 0, kb * 2, m * 2 + (int)rank, full + 8 * s);
+        };
+        const int pre = min(PAIR_STAGES, blocks);
+        int m, n;
+        tile_at(first, m_tiles, n_tiles, m, n);
+        for (int i = 0; i < pre; ++i) load_w(i, i, n);
+        grid_dependency_wait();
+        for (int i = 0; i < pre; ++i) load_x(i, i, m);
+        int s = pre == PAIR_STAGES ? 0 : pre;
+        uint32_t phase = pre == PAIR_STAGES ? 0 : 1, free = 0;        // (a stage that was never filled counts as free: parity 1 passes)
+        bool ok = true;
+        for (int i = first; i < tiles && ok; i += step) {
+            tile_at(i, m_tiles, n_tiles, m, n);
+            for (int kb = i == first ? pre : 0; kb < blocks; ++kb) {
+                if (!free && !mbar_wait(bar_empty + 8 * s, phase)) { atomicExch(&failed, 1); ok = false; break; }
+                const int now = s;
+                if (++s == PAIR_STAGES) { s = 0; phase ^= 1; }
+                free = mbar_peek(bar_empty + 8 * s, phase);
+                load_w(now, kb, n);
+                load_x(now, kb, m);
+            }
+        }
+    } else if (warp == 1 && rank == 0 && elect_one()) {
+        grid_dependency_wait();
+        int next = 0, turn = 0;
+        uint32_t phase = 0, full = 0;
+        bool ok = true;
+        for (int i = first; i < tiles && ok; i += step, ++turn) {
+            if (turn > 0 && !mbar_wait(bar_drained, (turn - 1) & 1)) { atomicExch(&failed, 1); break; }
+            fence_after_sync();
+            for (int kb = 0; kb < blocks; ++kb) {
+                const int s = next;
+                if (!full && !mbar_wait(bar_full + 8 * s, phase)) { atomicExch(&failed, 1); ok = false; break; }
+                if (++next == PAIR_STAGES) { next = 0; phase ^= 1; }
+                full = mbar_peek(bar_full + 8 * next, phase);
+                fence_after_sync();
+                const uint32_t x = stage0 + s * PAIR_STAGE, w = x + X_BYTES, sc = scales0 + s * SCALE_BYTES;
+                const uint32_t tx = tmem + 256 + s * SCALE_COLS, tw = tx + 4;
+                pair_scales_to_tmem(tx, sc);
+                pair_scales_to_tmem(tw, sc + BLOCK_BYTES);
+                pair_scales_to_tmem(tw + 4, sc + 2 * BLOCK_BYTES);
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    pair_umma_block(tmem, smem_desc(x + g * 32), smem_desc(w + g * 32), block_desc<mx::ROWS>(256, 256, g), tx, tw, (kb > 0 || g > 0) ? 1u : 0u);
+                pair_commit(bar_empty + 8 * s);
+            }
+            pair_commit(bar_sums);
+            if (!ok) mbar_wait(bar_sums, turn & 1);                   // (no product is under way when the tensor memory goes)
+        }
+    } else if (warp >= 4) {
+        grid_dependency_wait();
+        const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane;
+        const uint32_t drained = in_cta(bar_drained, 0);
+        int turn = 0;
+        for (int i = first; i < tiles; i += step, ++turn) {
+            int m, n;
+            tile_at(i, m_tiles, n_tiles, m, n);
+            const bool there = mbar_wait_parked(bar_sums, turn & 1, &failed);
+            if (!__all_sync(0xffffffffu, there && *(volatile int*)&failed == 0)) { atomicExch(&failed, 1); break; }
+            fence_after_sync();
+            uint32_t v[COLS];
+#pragma unroll
+            for (int c = 0; c < COLS; c += 32) tmem_load32(v + c, tmem + ((uint32_t)(warp % 4 * 32) << 16) + half * COLS + c);
+            tmem_wait_load();
+            fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive_there(drained);
+            finish_run<COLS, EPI>(v, o, m * 256 + (int)rank * 128 + row, n * 256 + half * COLS, T, N, vec);
+        }
+    } else {
+        grid_dependency_wait();
+    }
+    __syncwarp();
+    fence_before_sync();
+    __syncthreads();
+    if (failed != 0) {                                                // what is still under way for either CTA ends in microseconds: it waits for milliseconds
+        if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
+        for (int i = 0; i < 1000; ++i) __nanosleep(10000);
+    }
+    cg::this_cluster().sync();                                        // neither leaves while the other's products or copies need it
+    if (warp == 0) pair_tmem_free(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -751,6 +886,33 @@ static int many_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc,
                          stream, 1, mw, mx, ws, xs, o, T, N, kp, m_tiles, n_tiles, vec);
 }
 
+template <int EPI>
+static int pair_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
+                        cudaStream_t stream) {
+    const int m_tiles = (T + 255) / 256, n_tiles = o.codes != nullptr ? padded(N / 2) / 128 : (N + 255) / 256;
+    if ((long long)m_tiles * n_tiles > 1 << 30) return fail("mx_product: too many tiles");
+    const int cols = EPI == EPI_NONE ? N : N / 2, piece = o.dtype == JANIS_BF16 ? 8 : 4;
+    const int vec = cols % piece == 0 && ((uintptr_t)o.values & 15) == 0;
+    CUtensorMap mw, mx, mws, mxs;
+    if (!make_map(&mw, WEIGHTS, wc, N, kp, 128) || !make_map(&mx, ROWS, xc, T, kp, 128) ||
+        !make_scales_map(&mws, ws, (N + 127) / 128, kp / BLOCK, 2) || !make_scales_map(&mxs, xs, (T + 127) / 128, kp / BLOCK, 1))
+        return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
+    static std::once_flag once;
+    static cudaError_t e = cudaSuccess;
+    std::call_once(once, [] { e = cudaFuncSetAttribute(pair_rows_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM); });
+    if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
+    const int tiles = m_tiles * n_tiles, pairs = sm_count() / 2;
+    return launch_kernel("mx_product", pair_rows_kernel<EPI>, dim3(2 * (tiles < pairs ? tiles : pairs)), dim3(MANY_THREADS), PAIR_SMEM, stream, 2, mw, mx,
+                         mws, mxs, o, T, N, kp, m_tiles, n_tiles, vec);
+}
+
+static int pair_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp, cudaStream_t stream) {
+    if (o.epi == EPI_NONE) return pair_rows_as<EPI_NONE>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_GELU) return pair_rows_as<EPI_GATED_GELU>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_SILU) return pair_rows_as<EPI_GATED_SILU>(xc, xs, wc, ws, o, T, N, kp, stream);
+    return pair_rows_as<EPI_GATED_CLAMP>(xc, xs, wc, ws, o, T, N, kp, stream);
+}
+
 template <int SPLIT, int EPI>
 static int shared_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                           cudaStream_t stream) {
@@ -854,7 +1016,8 @@ using namespace janis;
 static int g_kernel = 0;
 
 // Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 that of many with 256 and 128 rows of W a tile, 4 that of
-// many whose K is shared (by the CTAs of janis_mx_set_few), 5, 6 and 7 the same by 2, 4 and 8.  For tests and tuning.
+// many whose K is shared (by the CTAs of janis_mx_set_few), 5, 6 and 7 the same by 2, 4 and 8, 8 that
+// of many by pairs of CTAs.  For tests and tuning.
 JANIS_EXPORT void janis_mx_set_kernel(int kernel) { g_kernel = kernel; }
 
 static int g_split = 0, g_stages = 0;
@@ -897,6 +1060,7 @@ JANIS_EXPORT int janis_mx_product(const void* block) {
     const int kp = mx::padded(K);
     const int kernel = g_kernel != 0 ? g_kernel : mx::choose(T, N, kp / mx::BLOCK, o);
     if (kernel == 1) return mx::few_rows(xc, xs, wc, ws, o, T, N, kp, g_split, g_stages, stream);
+    if (kernel == 8) return mx::pair_rows(xc, xs, wc, ws, o, T, N, kp, stream);
     if (kernel >= 5) return mx::shared_rows(1 << (kernel - 4), xc, xs, wc, ws, o, T, N, kp, stream);
     if (kernel == 4) return mx::shared_rows(g_split > 1 ? g_split : 2, xc, xs, wc, ws, o, T, N, kp, stream);
     return kernel == 2 ? mx::many_rows<256>(xc, xs, wc, ws, o, T, N, kp, stream) : mx::many_rows<128>(xc, xs, wc, ws, o, T, N, kp, stream);
