@@ -12,8 +12,8 @@
 //     waits for anybody else at the end.
 //
 // Many rows (prompts): bound by the tensor cores.
-//   * 128 rows of x are the M side, 256 (or 128) rows of W the N side, so that a thread of the epilogue has a row of x and a run of columns:
-//     gates beside their ups, whole groups of 32 for 8-bit rows, whole 16-byte pieces to store.
+//   * 128 rows of x are the M side, 128 rows of W the N side (256 and 256 of a pair of CTAs, which share one product), so that a thread of the
+//     epilogue has a row of x and a run of columns: gates beside their ups, whole groups of 32 for 8-bit rows, whole sectors to store.
 //   * A CTA an SM takes tile after tile.  One thread asks for the copies, one issues the products, eight warps drain: they take the sums
 //     into registers at once (half of the columns each four warps), give the tensor memory back and work while the next tile is multiplied.
 //
@@ -55,17 +55,18 @@ __device__ __forceinline__ float gated(float gate, float up, int epi, const Out&
 constexpr int TILE = 128;                      // rows of W a CTA
 constexpr int A_BYTES = TILE * 128, A_PACKED = A_BYTES / 2;
 constexpr int MAX_STAGES = 11;
-constexpr int MAX_ROWS = 256;                  // rows of x a CTA
-constexpr int SCALE_BYTES = 3 * BLOCK_BYTES;   // of a stage: a block of W's, one or two of x's
-constexpr int SCALE_COLS = 12;
+constexpr int FEW = 64;                        // rows of x at most
+constexpr int SCALE_BYTES = 2 * BLOCK_BYTES;   // of a stage: a block of W's, a block of x's
+constexpr int SCALE_COLS = 8;                  // of tensor memory
 constexpr int few_smem(int stages, int NP, int split) {
     return stages * (A_BYTES + NP * 128 + SCALE_BYTES) + 1024 + (split > 1 ? NP * TILE * 4 : 0);
 }
 
-// The end of a tile of few rows: sums [SPLIT][rows][128 / SPLIT] of rows of W from row0 on, by 128 threads.
+// The end of a tile of few rows: sums [SPLIT][rows][128 / SPLIT] of rows of W from row0 on, by the CTA's 128 threads.
 template <int SPLIT>
-__device__ __forceinline__ void store_rows(const float* sums, int rows, int t0, int row0, int id, int N, const Out& o) {
+__device__ __forceinline__ void store_rows(const float* sums, int rows, int row0, int N, const Out& o) {
     constexpr int SHARE = TILE / SPLIT;
+    const int id = threadIdx.x;
     const auto sum_at = [&](int m, int row) {                         // in the order of the ranks
         float v = sums[m * SHARE + row];
 #pragma unroll
@@ -77,8 +78,8 @@ __device__ __forceinline__ void store_rows(const float* sums, int rows, int t0, 
         if (n >= N) return;
         for (int m = id / SHARE; m < rows; m += SPLIT) {
             const float v = sum_at(m, row);
-            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * N + n] = from_float<bf16>(v);
-            else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * N + n] = v;
+            if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)m * N + n] = from_float<bf16>(v);
+            else reinterpret_cast<float*>(o.values)[(size_t)m * N + n] = v;
         }
         return;
     }
@@ -101,8 +102,8 @@ __device__ __forceinline__ void store_rows(const float* sums, int rows, int t0, 
             for (int u = 0; u < AT_ONCE; ++u) {
                 const int m = m0 + u * STEP;
                 if (m >= rows) break;
-                if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)(t0 + m) * all + c] = from_float<bf16>(v[u]);
-                else reinterpret_cast<float*>(o.values)[(size_t)(t0 + m) * all + c] = v[u];
+                if (o.dtype == JANIS_BF16) reinterpret_cast<bf16*>(o.values)[(size_t)m * all + c] = from_float<bf16>(v[u]);
+                else reinterpret_cast<float*>(o.values)[(size_t)m * all + c] = v[u];
             }
             continue;
         }
@@ -115,8 +116,8 @@ __device__ __forceinline__ void store_rows(const float* sums, int rows, int t0, 
             const int m = m0 + u * STEP;
             if (m >= rows) break;
             const uint32_t byte = scale_byte_e4m3(big[u]);
-            o.codes[(size_t)(t0 + m) * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v[u] * inverse_scale(byte), 0.f);
-            if ((id & 31) == 0) o.scales[scale_at(t0 + m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
+            o.codes[(size_t)m * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v[u] * inverse_scale(byte), 0.f);
+            if ((id & 31) == 0) o.scales[scale_at(m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
         }
     }
 }
@@ -132,14 +133,14 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     __shared__ int failed, asked;                                     // asked: stages that copies were asked for
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = SPLIT > 1 ? (int)cg::this_cluster().block_rank() : 0;
-    const int n0 = blockIdx.x / SPLIT * TILE, t0 = blockIdx.y * NP;
-    const int blocks = kp / BLOCK, rows = min(T - t0, NP);
+    const int n0 = blockIdx.x / SPLIT * TILE;
+    const int blocks = kp / BLOCK;
 
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
     const uint32_t stage0 = (raw + 1023) & ~1023u;                   // swizzle atoms want 1024-byte alignment
     const int stage_bytes = A_BYTES + NP * 128;
     const uint32_t scales0 = stage0 + stages * stage_bytes;
-    // [SPLIT][rows][SHARE] sums: behind the stages where others write them, over the idle stages where this CTA does
+    // [SPLIT][T][SHARE] sums: behind the stages where others write them, over the idle stages where this CTA does
     const uint32_t sums0 = SPLIT > 1 ? scales0 + stages * SCALE_BYTES : stage0;
     float* sums = reinterpret_cast<float*>(smem_raw + (sums0 - raw));
     const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
@@ -151,7 +152,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         mbar_init(bar_sums, 1);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-        if (SPLIT > 1) mbar_expect_tx(bar_sums, rows * TILE * 4);
+        if (SPLIT > 1) mbar_expect_tx(bar_sums, T * TILE * 4);
     }
     if (warp == 0) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), tmem_cols);
     fence_before_sync();
@@ -162,25 +163,22 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
     // this CTA's share of K: value blocks rank, rank + SPLIT, ...
     const int nk = (blocks - rank + SPLIT - 1) / SPLIT;
-    const int x_blocks = NP > BLOCK && t0 + BLOCK < T ? 2 : 1;       // blocks of x's scales that are there
     // (a tile past W's rows, which only makes the padding of 8-bit rows, finds zeros there whatever their scales)
     const uint8_t* w_scales = ws + (size_t)min(n0 / BLOCK, (N - 1) / BLOCK) * blocks * BLOCK_BYTES;
-    const uint8_t* x_scales = xs + (size_t)(t0 / BLOCK) * blocks * BLOCK_BYTES;
 
     grid_dependents_launch();
     if (warp == 0 && elect_one()) {
         // ---- the copies.  The weights are constants of the model: the first tiles of W are on their way before this kernel
         // waits for the one that makes x.
-        const int bytes = A_PACKED + NP * 128 + (1 + x_blocks) * BLOCK_BYTES;
+        const int bytes = A_PACKED + NP * 128 + 2 * BLOCK_BYTES;
         const auto load_w = [&](int kb, int s) {
             mbar_expect_tx(bar_full + 8 * s, bytes);
             tma_load_2d(stage0 + s * stage_bytes, &map_w, kb * BLOCK, n0, bar_full + 8 * s);
             bulk_load(scales0 + s * SCALE_BYTES, w_scales + (size_t)kb * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
         };
         const auto load_x = [&](int kb, int s) {
-            tma_load_2d(stage0 + s * stage_bytes + A_BYTES, &map_x, kb * BLOCK, t0, bar_full + 8 * s);
-            for (int b = 0; b < x_blocks; ++b)
-                bulk_load(scales0 + s * SCALE_BYTES + (1 + b) * BLOCK_BYTES, x_scales + ((size_t)b * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
+            tma_load_2d(stage0 + s * stage_bytes + A_BYTES, &map_x, kb * BLOCK, 0, bar_full + 8 * s);
+            bulk_load(scales0 + s * SCALE_BYTES + BLOCK_BYTES, xs + (size_t)kb * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
         };
         const int pre = nk < stages ? nk : stages;
         for (int i = 0; i < pre; ++i) load_w(rank + i * SPLIT, i);
@@ -212,7 +210,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
             const uint32_t a = stage0 + s * stage_bytes, b = a + A_BYTES, sc = scales0 + s * SCALE_BYTES;
             const uint32_t ta = tmem + NP + s * SCALE_COLS, tb = ta + 4;
             scales_to_tmem(ta, sc);
-            for (int j = 0; j < x_blocks; ++j) scales_to_tmem(tb + 4 * j, sc + (1 + j) * BLOCK_BYTES);
+            scales_to_tmem(tb, sc + BLOCK_BYTES);
 #pragma unroll
             for (int g = 0; g < 4; ++g)                               // 32 bytes further along the swizzled row
                 umma_block(tmem, smem_desc(a + g * 32), smem_desc(b + g * 32), block_desc<WEIGHTS>(TILE, NP, g), ta, tb, (i > 0 || g > 0) ? 1u : 0u);
@@ -231,19 +229,19 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (SPLIT > 1) asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory");      // everybody's barriers are there
 
     // ---- sums of row (32 * warp + lane) of the tile of W, to the CTA that adds them up
-    const uint32_t mine = sums0 + (uint32_t)(rank * rows * SHARE + threadIdx.x % SHARE) * 4;
+    const uint32_t mine = sums0 + (uint32_t)(rank * T * SHARE + threadIdx.x % SHARE) * 4;
     uint32_t there = mine, there_bar = bar_sums;
     if (SPLIT > 1) {
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there) : "r"(mine), "r"((uint32_t)threadIdx.x / SHARE));
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(there_bar) : "r"(bar_sums), "r"((uint32_t)threadIdx.x / SHARE));
     }
-    for (int c = 0; c < rows; c += 16) {
+    for (int c = 0; c < T; c += 16) {
         uint32_t r[16];
         tmem_load16(r, tmem + ((uint32_t)(warp * 32) << 16) + c);
         tmem_wait_load();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            if (c + j >= rows) break;
+            if (c + j >= T) break;
             if (SPLIT > 1)
                 asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];\n" ::"r"(there + (uint32_t)(c + j) * SHARE * 4),
                              "r"(r[j]), "r"(there_bar)
@@ -265,7 +263,13 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
         return;
     }
-    store_rows<SPLIT>(sums, rows, t0, n0 + rank * SHARE, threadIdx.x, N, o);
+    store_rows<SPLIT>(sums, T, n0 + rank * SHARE, N, o);
+}
+
+// how rows of out lie: 2 whole sectors, 1 whole 16 bytes, 0 neither
+static int pieces(const Out& o, int cols) {
+    const size_t row = (size_t)cols * (o.dtype == JANIS_BF16 ? 2 : 4), at = (uintptr_t)o.values;
+    return ((row | at) & 31) == 0 ? 2 : ((row | at) & 15) == 0 ? 1 : 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -273,9 +277,8 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 // ---------------------------------------------------------------------------
 constexpr int MANY_THREADS = 384;              // copies; products; two idle warps; two times four warps that drain
 constexpr int X_BYTES = 128 * 128;
-__host__ __device__ constexpr int many_stages(int BN) { return BN == 256 ? 4 : 6; }
-__host__ __device__ constexpr int many_buffers(int BN) { return BN == 256 ? 1 : 2; }      // of sums in tensor memory: 256 columns in all
-constexpr int many_smem(int BN) { return many_stages(BN) * (X_BYTES + BN * 128 + SCALE_BYTES) + 1024; }
+constexpr int MANY_STAGES = 6, MANY_STAGE = X_BYTES + A_BYTES, MANY_SCALES = 2 * BLOCK_BYTES;
+constexpr int MANY_SMEM = MANY_STAGES * (MANY_STAGE + MANY_SCALES) + 1024;
 constexpr int M_RUN = 16;                      // tiles of x that are taken with one tile of W after another
 
 __device__ __forceinline__ void tile_at(int i, int m_tiles, int n_tiles, int& m, int& n) {
@@ -284,45 +287,101 @@ __device__ __forceinline__ void tile_at(int i, int m_tiles, int n_tiles, int& m,
     m = run * M_RUN + within - n * height;
 }
 
-// `count` values of one row that lie together, at most those that the row has
+// 32 bytes of one lane: a whole sector of memory (16 bytes a lane, rows apart, write every sector twice)
+__device__ __forceinline__ void store_sector(void* p, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// SQUARE values of each of SQUARE lanes turned: afterwards lane l has value l of each of them.  Lanes K apart exchange what the other needs, then
+// K / 2 apart, ...
+template <int K, int SQUARE>
+__device__ __forceinline__ void turn_lanes(uint32_t* q) {
+    const bool up = (threadIdx.x & K) != 0;
+#pragma unroll
+    for (int b = 0; b < SQUARE; b += 2 * K)
+#pragma unroll
+        for (int i = b; i < b + K; ++i) {
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? q[i] : q[i + K], K);
+            q[i] = up ? got : q[i];
+            q[i + K] = up ? q[i + K] : got;
+        }
+    if constexpr (K > 1) turn_lanes<K / 2, SQUARE>(q);
+}
+
+// Columns c .. c + COUNT - 1 of row t of out [T, cols], of which this thread has the values; a whole warp calls it, and COUNT (at most 32) lanes
+// that lie together have rows that lie together.
+// vec 2: rows are whole sectors, 1: whole 16 bytes, 0: neither.  Then the values are turned among the lanes first,
+// so that a row's columns leave together.
 template <int COUNT>
-__device__ __forceinline__ void store_run(const uint32_t* v, const Out& o, size_t at, int left, bool vec) {
-    if (o.dtype == JANIS_BF16) {
-        bf16* p = reinterpret_cast<bf16*>(o.values) + at;
-        if (vec) {
+__device__ __forceinline__ void store_run(uint32_t* v, const Out& o, int t, int c, int T, int cols, int vec) {
+    const size_t at = (size_t)t * cols + c;
+    const int left = cols - c;
+    if (vec != 0) {
+        if (t >= T) return;
+        if (o.dtype == JANIS_BF16) {
+            bf16* p = reinterpret_cast<bf16*>(o.values) + at;
 #pragma unroll
             for (int j = 0; j < COUNT; j += 8)
                 if (j < left) {
-                    float f[8];
+                    if (COUNT % 16 == 0 && vec == 2) {
+                        if (j % 16 != 0) continue;
+                        uint32_t w[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j + e]);
-                    store_eight(p + j, f);
+                        for (int e = 0; e < 8; ++e) {
+                            const int k = COUNT % 16 == 0 ? j + 2 * e : 0;
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        store_sector(p + j, w);
+                    } else {
+                        float f[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(v[j + e]);
+                        store_eight(p + j, f);
+                    }
                 }
         } else {
-#pragma unroll
-            for (int j = 0; j < COUNT; ++j)
-                if (j < left) p[j] = from_float<bf16>(__uint_as_float(v[j]));
-        }
-    } else {
-        float* p = reinterpret_cast<float*>(o.values) + at;
-        if (vec) {
+            float* p = reinterpret_cast<float*>(o.values) + at;
 #pragma unroll
             for (int j = 0; j < COUNT; j += 4)
-                if (j < left) *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-        } else {
+                if (j < left) {
+                    if (vec == 2) {
+                        if (j % 8 == 0) store_sector(p + j, v + j);
+                    } else {
+                        *reinterpret_cast<uint4*>(p + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    }
+                }
+        }
+        return;
+    }
+    constexpr int SQUARE = COUNT < 32 ? COUNT : 32;
+    const int mine = threadIdx.x % SQUARE, rows = T - (t - mine);
 #pragma unroll
-            for (int j = 0; j < COUNT; ++j)
-                if (j < left) p[j] = __uint_as_float(v[j]);
+    for (int j = 0; j < COUNT; j += SQUARE) {
+        turn_lanes<SQUARE / 2, SQUARE>(v + j);                        // now of rows t - mine, t - mine + 1, ..., column c + j + mine
+        if (j + mine >= left) continue;
+        const size_t first = (size_t)(t - mine) * cols + c + j + mine;
+        if (o.dtype == JANIS_BF16) {
+            bf16* p = reinterpret_cast<bf16*>(o.values) + first;
+#pragma unroll
+            for (int i = 0; i < SQUARE; ++i, p += cols)
+                if (i < rows) *p = from_float<bf16>(__uint_as_float(v[j + i]));
+        } else {
+            float* p = reinterpret_cast<float*>(o.values) + first;
+#pragma unroll
+            for (int i = 0; i < SQUARE; ++i, p += cols)
+                if (i < rows) *p = __uint_as_float(v[j + i]);
         }
     }
 }
 
-// The end of a row's run of COLS columns of sums from column n0 on (rows of W), by the thread that holds them.
+// The end of a row's run of COLS columns of sums from column n0 on (rows of W), by the thread that holds them; a whole warp calls it.
 template <int COLS, int EPI>
-__device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, int t, int n0, int T, int N, bool vec) {
-    if (t >= T) return;
+__device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, int t, int n0, int T, int N, int vec) {
     if constexpr (EPI == EPI_NONE) {
-        store_run<COLS>(v, o, (size_t)t * N + n0, N - n0, vec);
+        store_run<COLS>(v, o, t, n0, T, N, vec);
     } else {
         const int cols = N / 2, wide = o.codes != nullptr ? padded(cols) : cols, c = n0 / 2;
 #pragma unroll
@@ -331,9 +390,10 @@ __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, in
             for (int j = 0; j < 8; ++j)
                 v[u * 8 + j] = __float_as_uint(gated(__uint_as_float(v[u * 16 + j]), __uint_as_float(v[u * 16 + 8 + j]), EPI, o));
         if (o.codes == nullptr) {
-            store_run<COLS / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
+            store_run<COLS / 2>(v, o, t, c, T, cols, vec);
             return;
         }
+        if (t >= T) return;
 #pragma unroll
         for (int g = 0; g < COLS / 64; ++g) {                         // (columns past the end are products with zeros)
             float big = 0.f;
@@ -351,35 +411,32 @@ __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, in
             }
             const int cg = c + g * 32;
             if (cg < wide) {
-                uint4* to = reinterpret_cast<uint4*>(o.codes + (size_t)t * wide + cg);
-                to[0] = make_uint4(q[0], q[1], q[2], q[3]);
-                to[1] = make_uint4(q[4], q[5], q[6], q[7]);
+                store_sector(o.codes + (size_t)t * wide + cg, q);
                 o.scales[scale_at(t, cg / BLOCK, wide / BLOCK) + cg % BLOCK / GROUP] = (uint8_t)byte;
             }
         }
     }
 }
 
-template <int BN, int EPI>
+template <int EPI>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
                  const uint8_t* __restrict__ xs, const Out o, int T, int N, int kp, int m_tiles, int n_tiles, int vec) {
-    constexpr int STAGES = many_stages(BN), BUFFERS = many_buffers(BN), STAGE = X_BYTES + BN * 128, W_BLOCKS = BN / BLOCK;
-    constexpr int COLS = BN / 2;                                      // columns of a draining warp
+    constexpr int COLS = 64;                                          // columns of a draining warp
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * STAGES + 2 * BUFFERS];
+    __shared__ __align__(8) unsigned long long bars[2 * MANY_STAGES + 4];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed, asked;                                     // asked: stages that copies were asked for
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blocks = kp / BLOCK, tiles = m_tiles * n_tiles;
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
-    const uint32_t stage0 = (raw + 1023) & ~1023u, scales0 = stage0 + STAGES * STAGE;
+    const uint32_t stage0 = (raw + 1023) & ~1023u, scales0 = stage0 + MANY_STAGES * MANY_STAGE;
     const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
-    const uint32_t bar_empty = bar_full + 8 * STAGES, bar_sums = bar_full + 16 * STAGES, bar_drained = bar_sums + 8 * BUFFERS;
+    const uint32_t bar_empty = bar_full + 8 * MANY_STAGES, bar_sums = bar_full + 16 * MANY_STAGES, bar_drained = bar_sums + 16;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * STAGES + BUFFERS; ++i) mbar_init(bar_full + 8 * i, 1);
-        for (int i = 0; i < BUFFERS; ++i) mbar_init(bar_drained + 8 * i, 8);
+        for (int i = 0; i < 2 * MANY_STAGES + 2; ++i) mbar_init(bar_full + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(bar_drained + 8 * i, 8);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -392,37 +449,34 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 
     if (warp == 0 && elect_one()) {
         const int w_last = (N - 1) / BLOCK;
-        const auto load_w = [&](int s, int kb, int n0) {
-            mbar_expect_tx(bar_full + 8 * s, X_BYTES + BN * 64 + (1 + W_BLOCKS) * BLOCK_BYTES);
-            tma_load_2d(stage0 + s * STAGE + X_BYTES, &map_w, kb * BLOCK, n0, bar_full + 8 * s);
-#pragma unroll
-            for (int b = 0; b < W_BLOCKS; ++b)                        // (what is past W's rows is zeros whatever their scales)
-                bulk_load(scales0 + s * SCALE_BYTES + (1 + b) * BLOCK_BYTES, ws + ((size_t)min(n0 / BLOCK + b, w_last) * blocks + kb) * BLOCK_BYTES,
-                          BLOCK_BYTES, bar_full + 8 * s);
+        const auto load_w = [&](int s, int kb, int n) {               // (what is past W's rows is zeros whatever their scales)
+            mbar_expect_tx(bar_full + 8 * s, X_BYTES + A_PACKED + 2 * BLOCK_BYTES);
+            tma_load_2d(stage0 + s * MANY_STAGE + X_BYTES, &map_w, kb * BLOCK, n * 128, bar_full + 8 * s);
+            bulk_load(scales0 + s * MANY_SCALES + BLOCK_BYTES, ws + ((size_t)min(n, w_last) * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
         };
         const auto load_x = [&](int s, int kb, int m) {
-            tma_load_2d(stage0 + s * STAGE, &map_x, kb * BLOCK, m * 128, bar_full + 8 * s);
-            bulk_load(scales0 + s * SCALE_BYTES, xs + ((size_t)m * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
+            tma_load_2d(stage0 + s * MANY_STAGE, &map_x, kb * BLOCK, m * 128, bar_full + 8 * s);
+            bulk_load(scales0 + s * MANY_SCALES, xs + ((size_t)m * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
         };
         // the weights are constants of the model: the first ones are on their way before x is there
-        const int pre = min(STAGES, blocks);
+        const int pre = min(MANY_STAGES, blocks);
         int m, n;
         tile_at(blockIdx.x, m_tiles, n_tiles, m, n);
-        for (int i = 0; i < pre; ++i) load_w(i, i, n * BN);
+        for (int i = 0; i < pre; ++i) load_w(i, i, n);
         grid_dependency_wait();
         for (int i = 0; i < pre; ++i) load_x(i, i, m);
         int filled = pre;
-        int s = pre == STAGES ? 0 : pre;
-        uint32_t phase = pre == STAGES ? 0 : 1, free = 0;             // (a stage that was never filled counts as free: parity 1 passes)
+        int s = pre == MANY_STAGES ? 0 : pre;
+        uint32_t phase = pre == MANY_STAGES ? 0 : 1, free = 0;             // (a stage that was never filled counts as free: parity 1 passes)
         bool ok = true;
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x) {
             tile_at(i, m_tiles, n_tiles, m, n);
             for (int kb = i == blockIdx.x ? pre : 0; kb < blocks; ++kb, ++filled) {
                 if (!free && !mbar_wait(bar_empty + 8 * s, phase)) { atomicExch(&failed, 1); ok = false; break; }
                 const int now = s;
-                if (++s == STAGES) { s = 0; phase ^= 1; }
+                if (++s == MANY_STAGES) { s = 0; phase ^= 1; }
                 free = mbar_peek(bar_empty + 8 * s, phase);
-                load_w(now, kb, n * BN);
+                load_w(now, kb, n);
                 load_x(now, kb, m);
             }
         }
@@ -433,48 +487,47 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 0, full = 0;
         bool ok = true;
         for (int i = blockIdx.x; i < tiles && ok; i += gridDim.x, ++turn) {
-            const int b = turn % BUFFERS;
-            const uint32_t d = tmem + b * BN;
-            if (turn >= BUFFERS && !mbar_wait(bar_drained + 8 * b, (turn / BUFFERS - 1) & 1)) { atomicExch(&failed, 1); break; }
+            const int b = turn & 1;
+            const uint32_t d = tmem + b * 128;
+            if (turn >= 2 && !mbar_wait(bar_drained + 8 * b, (turn / 2 - 1) & 1)) { atomicExch(&failed, 1); break; }
             fence_after_sync();
             for (int kb = 0; kb < blocks; ++kb) {
                 const int s = next;
                 if (!full && !mbar_wait(bar_full + 8 * s, phase)) { atomicExch(&failed, 1); ok = false; break; }
-                if (++next == STAGES) { next = 0; phase ^= 1; }
+                if (++next == MANY_STAGES) { next = 0; phase ^= 1; }
                 full = mbar_peek(bar_full + 8 * next, phase);
                 fence_after_sync();
-                const uint32_t x = stage0 + s * STAGE, w = x + X_BYTES, sc = scales0 + s * SCALE_BYTES;
-                const uint32_t tx = tmem + 256 + s * SCALE_COLS, tw = tx + 4;
+                const uint32_t x = stage0 + s * MANY_STAGE, w = x + X_BYTES, sc = scales0 + s * MANY_SCALES;
+                const uint32_t tx = tmem + 256 + s * 8, tw = tx + 4;
                 scales_to_tmem(tx, sc);
-#pragma unroll
-                for (int j = 0; j < W_BLOCKS; ++j) scales_to_tmem(tw + 4 * j, sc + (1 + j) * BLOCK_BYTES);
+                scales_to_tmem(tw, sc + BLOCK_BYTES);
 #pragma unroll
                 for (int g = 0; g < 4; ++g)
-                    umma_block(d, smem_desc(x + g * 32), smem_desc(w + g * 32), block_desc<ROWS>(128, BN, g), tx, tw, (kb > 0 || g > 0) ? 1u : 0u);
+                    umma_block(d, smem_desc(x + g * 32), smem_desc(w + g * 32), block_desc<ROWS>(128, 128, g), tx, tw, (kb > 0 || g > 0) ? 1u : 0u);
                 umma_commit(bar_empty + 8 * s);
             }
             umma_commit(bar_sums + 8 * b);
-            if (!ok) mbar_wait(bar_sums + 8 * b, (turn / BUFFERS) & 1);      // (no product is under way when the tensor memory goes)
+            if (!ok) mbar_wait(bar_sums + 8 * b, (turn / 2) & 1);      // (no product is under way when the tensor memory goes)
         }
     } else if (warp >= 4) {
         grid_dependency_wait();
         const int half = (warp - 4) / 4, row = warp % 4 * 32 + lane;  // (a warp reaches the quarter of tensor memory that its number says)
         int turn = 0;
         for (int i = blockIdx.x; i < tiles; i += gridDim.x, ++turn) {
-            const int b = turn % BUFFERS;
+            const int b = turn & 1;
             int m, n;
             tile_at(i, m_tiles, n_tiles, m, n);
-            const bool there = mbar_wait_parked(bar_sums + 8 * b, (turn / BUFFERS) & 1, &failed);
+            const bool there = mbar_wait_parked(bar_sums + 8 * b, (turn / 2) & 1, &failed);
             if (!__all_sync(0xffffffffu, there && *(volatile int*)&failed == 0)) { atomicExch(&failed, 1); break; }
             fence_after_sync();
             uint32_t v[COLS];
 #pragma unroll
-            for (int c = 0; c < COLS; c += 32) tmem_load32(v + c, tmem + ((uint32_t)(warp % 4 * 32) << 16) + b * BN + half * COLS + c);
+            for (int c = 0; c < COLS; c += 32) tmem_load32(v + c, tmem + ((uint32_t)(warp % 4 * 32) << 16) + b * 128 + half * COLS + c);
             tmem_wait_load();
             fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_drained + 8 * b);
-            finish_run<COLS, EPI>(v, o, m * 128 + row, n * BN + half * COLS, T, N, vec);
+            finish_run<COLS, EPI>(v, o, m * 128 + row, n * 128 + half * COLS, T, N, vec);
         }
     } else {
         grid_dependency_wait();
@@ -484,7 +537,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
     __syncthreads();
     if (failed != 0 && threadIdx.x == 0) {                            // no copy is under way when the CTA leaves
         atomicAdd(&g_timeouts, 1);
-        for (int j = asked > STAGES ? asked - STAGES : 0; j < asked; ++j) mbar_wait(bar_full + 8 * (j % STAGES), (j / STAGES) & 1);
+        for (int j = asked > MANY_STAGES ? asked - MANY_STAGES : 0; j < asked; ++j) mbar_wait(bar_full + 8 * (j % MANY_STAGES), (j / MANY_STAGES) & 1);
     }
     if (warp == 0) tmem_free(tmem, 512);
 }
@@ -492,16 +545,19 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 // ---------------------------------------------------------------------------
 // many rows, two CTAs as one
 // ---------------------------------------------------------------------------
-constexpr int PAIR_STAGES = 6, PAIR_STAGE = X_BYTES + A_BYTES;
-constexpr int PAIR_SMEM = PAIR_STAGES * (PAIR_STAGE + SCALE_BYTES) + 1024;
+constexpr int PAIR_STAGES = 6, PAIR_STAGE = X_BYTES + A_BYTES, PAIR_SCALES = 3 * BLOCK_BYTES, PAIR_COLS = 12;
+constexpr int PAIR_SMEM = PAIR_STAGES * (PAIR_STAGE + PAIR_SCALES) + 1024;
 
 // 256 rows of x by 256 of W: each SM holds half of both, so that it fetches and reads two thirds of what a tile of 128 x 256 wants for the same
-// products, and its sums are 128 rows of 256 columns as there.
+// products, and its sums are 128 rows of 256 columns.  At prompts' sizes the products are bound by the power limit (1.1 to 1.5 GHz), so that what
+// a tile does not fetch counts: 2,048 rows x 4,608 x 36,864 254 us, against 274 with tiles of 128 x 256 of one SM and 333 of 128 x 128.
+// Tensor memory holds one tile's sums, and the products wait some 2 us while they are taken out.  Tiles of 256 x 192, of which it holds two, close
+// that gap and are no faster: 2,048 x 18,432 x 2,304 gated 74.5 us against 73.4, 2,048 x 4,608 x 36,864 281 against 255.
 template <int EPI>
 __global__ void __launch_bounds__(MANY_THREADS, 1)
 pair_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_ws,
                  const __grid_constant__ CUtensorMap map_xs, const Out o, int T, int N, int kp, int m_tiles, int n_tiles, int vec) {
-    constexpr int COLS = 128;
+    constexpr int COLS = 128;                                         // columns of a draining warp
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) unsigned long long bars[2 * PAIR_STAGES + 2];
     __shared__ uint32_t tmem_slot;
@@ -534,11 +590,11 @@ pair_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         const auto load_w = [&](int s, int kb, int n) {
             if (rank == 0) mbar_expect_tx(bar_full + 8 * s, 2 * (X_BYTES + A_PACKED + 3 * BLOCK_BYTES));
             pair_load_2d(stage0 + s * PAIR_STAGE + X_BYTES, &map_w, kb * BLOCK, n * 256 + (int)rank * 128, full + 8 * s);
-            pair_load_3d(scales0 + s * SCALE_BYTES + BLOCK_BYTES, &map_ws, 0, kb * 2, n * 2, full + 8 * s);
+            pair_load_3d(scales0 + s * PAIR_SCALES + BLOCK_BYTES, &map_ws, 0, kb * 2, n * 2, full + 8 * s);
         };
         const auto load_x = [&](int s, int kb, int m) {
             pair_load_2d(stage0 + s * PAIR_STAGE, &map_x, kb * BLOCK, m * 256 + (int)rank * 128, full + 8 * s);
-            pair_load_3d(scales0 + s * SCALE_BYTES, &map_xs, 0, kb * 2, m * 2 + (int)rank, full + 8 * s);
+            pair_load_3d(scales0 + s * PAIR_SCALES, &map_xs, 0, kb * 2, m * 2 + (int)rank, full + 8 * s);
         };
         const int pre = min(PAIR_STAGES, blocks);
         int m, n;
@@ -574,8 +630,8 @@ pair_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
                 if (++next == PAIR_STAGES) { next = 0; phase ^= 1; }
                 full = mbar_peek(bar_full + 8 * next, phase);
                 fence_after_sync();
-                const uint32_t x = stage0 + s * PAIR_STAGE, w = x + X_BYTES, sc = scales0 + s * SCALE_BYTES;
-                const uint32_t tx = tmem + 256 + s * SCALE_COLS, tw = tx + 4;
+                const uint32_t x = stage0 + s * PAIR_STAGE, w = x + X_BYTES, sc = scales0 + s * PAIR_SCALES;
+                const uint32_t tx = tmem + 256 + s * PAIR_COLS, tw = tx + 4;
                 pair_scales_to_tmem(tx, sc);
                 pair_scales_to_tmem(tw, sc + BLOCK_BYTES);
                 pair_scales_to_tmem(tw + 4, sc + 2 * BLOCK_BYTES);
@@ -773,7 +829,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
         v[c] = __float_as_uint(f);
     }
     if (EPI == EPI_NONE) {
-        if (live) store_run<RUN>(v, o, (size_t)t * N + n * 128 + c0, N - n * 128 - c0, vec);
+        store_run<RUN>(v, o, t, n * 128 + c0, T, N, vec);
         return;
     }
     if constexpr (EPI != EPI_NONE && RUN >= 16) {
@@ -784,7 +840,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             for (int j = 0; j < 8; ++j)
                 v[u * 8 + j] = __float_as_uint(gated(__uint_as_float(v[u * 16 + j]), __uint_as_float(v[u * 16 + 8 + j]), EPI, o));
         if (o.codes == nullptr) {
-            if (live) store_run<RUN / 2>(v, o, (size_t)t * cols + c, cols - c, vec);
+            store_run<RUN / 2>(v, o, t, c, T, cols, vec);
             return;
         }
         constexpr int HELD = RUN / 2, RUNS = 32 / HELD;               // columns of a thread: 16 or 8 of a group of 32, the others in other warps
@@ -821,31 +877,29 @@ static int sm_count() {
 
 static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                     int split, int stages, cudaStream_t stream) {
-    const int NP = T >= MAX_ROWS ? MAX_ROWS : (T + 15) / 16 * 16;
+    if (T > FEW) return fail("mx_product: at most %d rows in this kernel, found %d", FEW, T);
+    const int NP = (T + 15) / 16 * 16;
     // (8-bit rows are padded to whole blocks of 128 columns: 256 rows of gates and ups)
-    const int tiles = o.codes != nullptr ? padded(N / 2) / (TILE / 2) : (N + TILE - 1) / TILE, blocks = kp / BLOCK, t_tiles = (T + NP - 1) / NP;
+    const int tiles = o.codes != nullptr ? padded(N / 2) / (TILE / 2) : (N + TILE - 1) / TILE, blocks = kp / BLOCK;
     const int most_split = o.codes != nullptr ? 2 : 8;                // (a group of 8-bit rows lies within a CTA's share)
     if (split == 0) {
         // K is shared while all CTAs are resident, two an SM, and keep four blocks each.  A cluster lies within a GPC, of whose 16 to 18
         // SMs four clusters of 8 take all: 32 in all, or 48 of three CTAs an SM, which pay where K is long only.  One row, us with 1, 2, 4,
         // 8 CTAs: 2,304 x 2,048 5.3, 3.6, 2.9, 3.3; 4,096 x 2,304 5.8, 3.8, 3.4, 4.2; 2,304 x 9,216 18, 10, 6.4, 4.8; 18,432 x 2,304 7.2, 6.1;
         // 4,608 x 4,096 -, -, 4.4, 4.8 (36 tiles); 4,608 x 36,864 66, 34, 22, 20 (36 tiles).
-        const long long ctas = (long long)tiles * t_tiles;
         split = 1;
-        while (split < most_split && ctas * split * 2 <= (NP > 64 ? 1 : 2) * sm_count() && blocks >= split * 2 * 4 && (split < 4 || ctas <= 32)) split *= 2;
-        if (split == 4 && most_split == 8 && NP <= 32 && ctas > 32 && ctas <= 48 && blocks >= 128) split = 8;
+        while (split < most_split && tiles * split * 2 <= 2 * sm_count() && blocks >= split * 2 * 4 && (split < 4 || tiles <= 32)) split *= 2;
+        if (split == 4 && most_split == 8 && NP <= 32 && tiles > 32 && tiles <= 48 && blocks >= 128) split = 8;
     }
     if (split > most_split || split > blocks || (split & (split - 1)) != 0) return fail("mx_product: a split of %d is not possible here", split);
     const int most = 227 * 1024 - 512;
     if (stages == 0) {
         // a ring as deep as the SM's memory allows for the CTAs that share it
-        const long long ctas = (long long)tiles * t_tiles;
-        const int room = split == 8 && NP <= 32 && ctas > 32 ? 74 * 1024 : (split > 1 && NP <= 64) || ctas > sm_count() ? 113 * 1024 : most;
+        const int room = split == 8 && NP <= 32 && tiles > 32 ? 74 * 1024 : split > 1 || tiles > sm_count() ? 113 * 1024 : most;
         stages = (room - 1024 - (split > 1 ? NP * TILE * 4 : 0)) / (A_BYTES + NP * 128 + SCALE_BYTES);
         const int share = (blocks + split - 1) / split;
         if (stages > share) stages = share;
         if (stages > MAX_STAGES) stages = MAX_STAGES;
-        if (stages < 1) stages = 1;
         while (split == 1 && stages * (A_BYTES + NP * 128) < NP * TILE * 4) ++stages;      // (the sums leave through them)
     }
     if (stages < 1 || stages > MAX_STAGES || few_smem(stages, NP, split) > most || (split == 1 && stages * (A_BYTES + NP * 128) < NP * TILE * 4))
@@ -863,26 +917,25 @@ static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, con
             if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512);
     });
     if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
-    return launch_kernel("mx_product", kernel, dim3(tiles * split, t_tiles), dim3(128), few_smem(stages, NP, split), stream, split, mw, mx, ws, xs, o,
+    return launch_kernel("mx_product", kernel, dim3(tiles * split), dim3(128), few_smem(stages, NP, split), stream, split, mw, mx, ws, xs, o,
                          T, N, kp, NP, stages, cols);
 }
 
-template <int BN, int EPI>
+template <int EPI>
 static int many_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                         cudaStream_t stream) {
-    const int m_tiles = (T + 127) / 128, n_tiles = o.codes != nullptr ? (padded(N / 2) * 2 + BN - 1) / BN : (N + BN - 1) / BN;
+    const int m_tiles = (T + 127) / 128, n_tiles = o.codes != nullptr ? padded(N / 2) / 64 : (N + 127) / 128;
     if ((long long)m_tiles * n_tiles > 1 << 30) return fail("mx_product: too many tiles");
-    const int cols = EPI == EPI_NONE ? N : N / 2, piece = o.dtype == JANIS_BF16 ? 8 : 4;
-    const int vec = cols % piece == 0 && ((uintptr_t)o.values & 15) == 0;
+    const int vec = pieces(o, EPI == EPI_NONE ? N : N / 2);
     CUtensorMap mw, mx;
-    if (!make_map(&mw, WEIGHTS, wc, N, kp, BN) || !make_map(&mx, ROWS, xc, T, kp, 128))
+    if (!make_map(&mw, WEIGHTS, wc, N, kp, 128) || !make_map(&mx, ROWS, xc, T, kp, 128))
         return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
     static std::once_flag once;
     static cudaError_t e = cudaSuccess;
-    std::call_once(once, [] { e = cudaFuncSetAttribute(many_rows_kernel<BN, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, many_smem(BN)); });
+    std::call_once(once, [] { e = cudaFuncSetAttribute(many_rows_kernel<EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize, MANY_SMEM); });
     if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
     const int tiles = m_tiles * n_tiles;
-    return launch_kernel("mx_product", many_rows_kernel<BN, EPI>, dim3(tiles < sm_count() ? tiles : sm_count()), dim3(MANY_THREADS), many_smem(BN),
+    return launch_kernel("mx_product", many_rows_kernel<EPI>, dim3(tiles < sm_count() ? tiles : sm_count()), dim3(MANY_THREADS), MANY_SMEM,
                          stream, 1, mw, mx, ws, xs, o, T, N, kp, m_tiles, n_tiles, vec);
 }
 
@@ -891,8 +944,7 @@ static int pair_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc,
                         cudaStream_t stream) {
     const int m_tiles = (T + 255) / 256, n_tiles = o.codes != nullptr ? padded(N / 2) / 128 : (N + 255) / 256;
     if ((long long)m_tiles * n_tiles > 1 << 30) return fail("mx_product: too many tiles");
-    const int cols = EPI == EPI_NONE ? N : N / 2, piece = o.dtype == JANIS_BF16 ? 8 : 4;
-    const int vec = cols % piece == 0 && ((uintptr_t)o.values & 15) == 0;
+    const int vec = pieces(o, EPI == EPI_NONE ? N : N / 2);
     CUtensorMap mw, mx, mws, mxs;
     if (!make_map(&mw, WEIGHTS, wc, N, kp, 128) || !make_map(&mx, ROWS, xc, T, kp, 128) ||
         !make_scales_map(&mws, ws, (N + 127) / 128, kp / BLOCK, 2) || !make_scales_map(&mxs, xs, (T + 127) / 128, kp / BLOCK, 1))
@@ -917,8 +969,7 @@ template <int SPLIT, int EPI>
 static int shared_rows_as(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                           cudaStream_t stream) {
     const int m_tiles = (T + 127) / 128, n_tiles = o.codes != nullptr ? padded(N / 2) / 64 : (N + 127) / 128;
-    const int cols = EPI == EPI_NONE ? N : N / 2, piece = o.dtype == JANIS_BF16 ? 8 : 4;
-    const int vec = cols % piece == 0 && ((uintptr_t)o.values & 15) == 0;
+    const int vec = pieces(o, EPI == EPI_NONE ? N : N / 2);
     CUtensorMap mw, mx;
     if (!make_map(&mw, WEIGHTS, wc, N, kp, 128) || !make_map(&mx, ROWS, xc, T, kp, 128))
         return fail("mx_product: cuTensorMapEncodeTiled is not available or refused the operands");
@@ -974,23 +1025,27 @@ static int clusters_held() {
     return n;
 }
 
-// The kernel of a product: 1 few rows, 2 and 3 many with 256 and 128 rows of W a tile, 5, 6, 7 many whose K is shared by 2, 4, 8 CTAs.
+// The kernel of a product: 1 few rows, 2 and 3 many by pairs of CTAs and by one, 5, 6, 7 many whose K is shared by 2, 4, 8 CTAs.
 // Up to 64 rows the first (32 with a gated epilogue, which is the longer the more rows a thread has: 64 rows x 28,672 x 3,584 27.5 us against 17.4),
-// but where K is short (at 777, 1,000 weights and 32 rows 3.6 us against 3.1) or W alone fills the SMs (64 rows x 18,432 x
-// 2,304: 9.0 against 7.8).  Above, the least of what they take in us, as measured: a wave of tiles costs 0.22 a block of K and 1.2 at 128 rows of W,
-// 0.36 and 1.2 at 256, and 1.5 and 2.2 once; sharing costs 0.28 a block and 4.2, as long as all clusters are resident.
+// but where K is short (at 777, 1,000 weights and 32 rows 3.6 us against 3.1) or W alone fills the SMs (64 rows x 18,432 x 2,304: 9.0 against 7.8).
+// Above, the least of what they take in us, as measured: a wave of tiles costs 0.22 a block of K and 1.2 by one CTA, 0.30 and 2.3 by pairs (of twice
+// the rows and columns), and 1.5 and 2.5 once; sharing costs 0.28 a block and 4.2, as long as all clusters are resident.  So measured, by one CTA
+// and by pairs: 128 rows x 18,432 x 2,304 9.0, 12.9 us; 256 rows 14.0, 13.2; 2,048 rows 92.8, 77.0.  Rows of out that start anywhere add 1.9, 4.5 and
+// 0.5 once (128 rows x 777 x 1,000: 4.3 -> 6.2 by one CTA, 4.6 -> 4.9 by four that share).
 static int choose(int T, int N, int blocks, const Out& o) {
     const int sms = sm_count(), m_tiles = (T + 127) / 128;
-    const long long tiles128 = (long long)m_tiles * ((N + 127) / 128), tiles256 = (long long)m_tiles * ((N + 255) / 256);
-    if (T <= 16 || (T <= (o.epi == EPI_NONE ? 64 : 32) && blocks > 8 && !(T > 48 && tiles128 * 8 >= sms * 7))) return 1;
-    const double cost128 = (tiles128 + sms - 1) / sms * (0.22 * blocks + 1.2) + 1.5, cost256 = (tiles256 + sms - 1) / sms * (0.36 * blocks + 1.2) + 2.2;
-    int best = cost128 <= cost256 ? 3 : 2;
-    double least = cost128 <= cost256 ? cost128 : cost256;
+    const long long tiles128 = (long long)m_tiles * ((N + 127) / 128), pairs = (long long)((T + 255) / 256) * ((N + 255) / 256);
+    const bool anywhere = o.codes == nullptr && pieces(o, o.epi == EPI_NONE ? N : N / 2) == 0;
+    if (T <= 16 || (T <= (o.epi == EPI_NONE ? 64 : 32) && (blocks > 8 || anywhere) && !(T > 48 && tiles128 * 8 >= sms * 7))) return 1;
+    const double cost_one = (tiles128 + sms - 1) / sms * (0.22 * blocks + 1.2) + (anywhere ? 3.4 : 1.5);
+    const double cost_pair = (pairs + sms / 2 - 1) / (sms / 2) * (0.30 * blocks + 2.3) + (anywhere ? 7.0 : 2.5);
+    int best = cost_one <= cost_pair ? 3 : 2;
+    double least = cost_one <= cost_pair ? cost_one : cost_pair;
     const int held[3] = {tiles128 <= sms / 2 ? clusters_held<2>() : 0, tiles128 <= sms / 4 ? clusters_held<4>() : 0,
                          tiles128 <= sms / 8 && o.epi == EPI_NONE ? clusters_held<8>() : 0};
     for (int i = 0; i < 3; ++i) {
         const int split = 2 << i;
-        const double cost = 0.28 * ((blocks + split - 1) / split) + 4.2;
+        const double cost = 0.28 * ((blocks + split - 1) / split) + (anywhere ? 4.7 : 4.2);
         if (tiles128 <= held[i] && blocks >= 2 * split && cost < least) {
             best = 5 + i;
             least = cost;
@@ -999,13 +1054,12 @@ static int choose(int T, int N, int blocks, const Out& o) {
     return best;
 }
 
-template <int BN>
 static int many_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, const uint8_t* ws, const Out& o, int T, int N, int kp,
                      cudaStream_t stream) {
-    if (o.epi == EPI_NONE) return many_rows_as<BN, EPI_NONE>(xc, xs, wc, ws, o, T, N, kp, stream);
-    if (o.epi == EPI_GATED_GELU) return many_rows_as<BN, EPI_GATED_GELU>(xc, xs, wc, ws, o, T, N, kp, stream);
-    if (o.epi == EPI_GATED_SILU) return many_rows_as<BN, EPI_GATED_SILU>(xc, xs, wc, ws, o, T, N, kp, stream);
-    return many_rows_as<BN, EPI_GATED_CLAMP>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_NONE) return many_rows_as<EPI_NONE>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_GELU) return many_rows_as<EPI_GATED_GELU>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (o.epi == EPI_GATED_SILU) return many_rows_as<EPI_GATED_SILU>(xc, xs, wc, ws, o, T, N, kp, stream);
+    return many_rows_as<EPI_GATED_CLAMP>(xc, xs, wc, ws, o, T, N, kp, stream);
 }
 
 }  // namespace mx
@@ -1015,9 +1069,8 @@ using namespace janis;
 
 static int g_kernel = 0;
 
-// Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 that of many with 256 and 128 rows of W a tile, 4 that of
-// many whose K is shared (by the CTAs of janis_mx_set_few), 5, 6 and 7 the same by 2, 4 and 8, 8 that
-// of many by pairs of CTAs.  For tests and tuning.
+// Fixes the kernel of products: 0 chosen, 1 that of few rows, 2 and 3 those of many by pairs of CTAs and by one, 4 that of many whose K is shared by the
+// CTAs of janis_mx_set_few, 5, 6 and 7 the same by 2, 4 and 8.  For tests and tuning.
 JANIS_EXPORT void janis_mx_set_kernel(int kernel) { g_kernel = kernel; }
 
 static int g_split = 0, g_stages = 0;
@@ -1060,10 +1113,9 @@ JANIS_EXPORT int janis_mx_product(const void* block) {
     const int kp = mx::padded(K);
     const int kernel = g_kernel != 0 ? g_kernel : mx::choose(T, N, kp / mx::BLOCK, o);
     if (kernel == 1) return mx::few_rows(xc, xs, wc, ws, o, T, N, kp, g_split, g_stages, stream);
-    if (kernel == 8) return mx::pair_rows(xc, xs, wc, ws, o, T, N, kp, stream);
-    if (kernel >= 5) return mx::shared_rows(1 << (kernel - 4), xc, xs, wc, ws, o, T, N, kp, stream);
-    if (kernel == 4) return mx::shared_rows(g_split > 1 ? g_split : 2, xc, xs, wc, ws, o, T, N, kp, stream);
-    return kernel == 2 ? mx::many_rows<256>(xc, xs, wc, ws, o, T, N, kp, stream) : mx::many_rows<128>(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (kernel == 2) return mx::pair_rows(xc, xs, wc, ws, o, T, N, kp, stream);
+    if (kernel == 3) return mx::many_rows(xc, xs, wc, ws, o, T, N, kp, stream);
+    return mx::shared_rows(kernel > 4 ? 1 << (kernel - 4) : g_split > 1 ? g_split : 2, xc, xs, wc, ws, o, T, N, kp, stream);
 }
 
 // The count of given-up waits copied into `host` (pinned memory, two ints, the second always 0) in the order of `stream`.
