@@ -254,7 +254,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     if (SPLIT > 1) {
         // (others may be at their own waits' limits: this CTA's memory has to outlast what they send)
         bool all = false;
-        for (int i = 0; i < 8 && !all; ++i) all = mbar_wait(bar_sums, 0);
+        for (int i = 0; i < 8 && !all; ++i) all = mbar_wait_cluster(bar_sums, 0);
         ok = ok && all;
     }
     ok = __syncthreads_and(ok ? 1 : 0);
@@ -622,7 +622,7 @@ pair_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
         uint32_t phase = 0, full = 0;
         bool ok = true;
         for (int i = first; i < tiles && ok; i += step, ++turn) {
-            if (turn > 0 && !mbar_wait(bar_drained, (turn - 1) & 1)) { atomicExch(&failed, 1); break; }
+            if (turn > 0 && !mbar_wait_cluster(bar_drained, (turn - 1) & 1)) { atomicExch(&failed, 1); break; }
             fence_after_sync();
             for (int kb = 0; kb < blocks; ++kb) {
                 const int s = next;
@@ -806,7 +806,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     {
         // (others may be at their own waits' limits: this CTA's memory has to outlast what they send)
         bool all = false;
-        for (int i = 0; i < 8 && !all; ++i) all = mbar_wait(bar_sums, 0);
+        for (int i = 0; i < 8 && !all; ++i) all = mbar_wait_cluster(bar_sums, 0);
         ok = ok && all;
     }
     ok = __syncthreads_and(ok ? 1 : 0);
@@ -1118,7 +1118,7 @@ JANIS_EXPORT int janis_mx_product(const void* block) {
     return mx::shared_rows(kernel > 4 ? 1 << (kernel - 4) : g_split > 1 ? g_split : 2, xc, xs, wc, ws, o, T, N, kp, stream);
 }
 
-// The count of given-up waits copied into `host` (pinned memory, two ints, the second always 0) in the order of `stream`.
+// The count of given-up waits copied into `host` (pinned memory, one int) in the order of `stream`.
 JANIS_EXPORT int janis_mx_timeouts_async(int* host, cudaStream_t stream) {
     cudaError_t e = cudaMemcpyFromSymbolAsync(host, mx::g_timeouts, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
     if (e != cudaSuccess) return fail("mx_timeouts_async: %s", cudaGetErrorString(e));

@@ -186,7 +186,8 @@ def mx_set_kernel(kernel: int = 0) -> None:
 def linear_mx(x: MxRows, w: MxWeight, out, epilogue: int = 0, limit: float = 0.0, alpha: float = 1.0, up_add: float = 0.0):
     """out[T, N] = x w^T of 8-bit rows and 4-bit weights, float sums; out bfloat16 or float32.  With a gated epilogue
     (EPI_GATED_GELU, EPI_GATED_SILU, EPI_GATED_CLAMP with its three numbers) the rows of w alternate 8 gates, 8 ups and
-    out[T, N / 2] = act(gate) * up; it may be `MxRows` then."""
+    out[T, N / 2] = act(gate) * up; it may be `MxRows` then.  Like every product of this library it takes w for a constant: its first
+    tiles are fetched while the kernel in front of this one still runs."""
     if type(x) is not MxRows or type(w) is not MxWeight:
         raise _ops.KernelError(f"linear_mx: x must be MxRows and w MxWeight, found {type(x).__name__} and {type(w).__name__}")
     T, K, N = x.rows, x.width, w.rows
