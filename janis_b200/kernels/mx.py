@@ -199,8 +199,10 @@ def linear_mx(x: MxRows, w: MxWeight, out, epilogue: int = 0, limit: float = 0.0
             raise _ops.KernelError("linear_mx: 8-bit rows are a gated epilogue's output")
         p_out, dt, (pc, ps) = 0, 0, _rows(out, "out", T, cols)
     else:
-        p_out, pc, ps = _ops._t(out, "out", _ops._FLOATS, (T, cols)), 0, 0
-        dt = _ops._DT[out.dtype]
+        dt = _ops._DT.get(getattr(out, "dtype", None))
+        if dt is None or out.shape != (T, cols) or not out.is_cuda or not out.is_contiguous():
+            _ops._t(out, "out", _ops._FLOATS, (T, cols))                  # (says what is wrong with it)
+        p_out, pc, ps = out.data_ptr(), 0, 0
     lib = _ops._low_bits or _ops.low_bits()
     _ops._check(lib, lib.janis_mx_product(_PRODUCT(
         x.codes.data_ptr(), x.scales.data_ptr(), w.codes.data_ptr(), w.scales.data_ptr(), p_out, dt, pc, ps, T, N, K, epilogue,

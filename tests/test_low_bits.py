@@ -423,6 +423,33 @@ def test_another_stream_and_no_rows():
 
 
 @GPU
+def test_offsets_that_pass_32_bits():
+    """Rows of x, of out and of the stream whose places pass 2^31 values; all but the last few are zeros."""
+    o = ops()
+    last, t = 5, 70016
+    for n, k in ((256, 36864), (32768, 128)):                # x of 2.6e9 codes; out of 2.3e9 values
+        x, w = o.MxRows.empty(t, k), o.mx_weight(rnd(n, k) / math.sqrt(k))
+        tail, _ = operands(last, 1, k, seed=3)
+        x.codes[-last:] = tail.codes
+        r, g = torch.arange(t - last, t, device="cuda")[:, None], torch.arange(k // 32, device="cuda")
+        x.scales.view(-1)[(r // 128 * (k // 128) + g // 4) * 512 + r % 32 * 16 + r % 128 // 32 * 4 + g % 4] = scale_rows(tail)
+        out = o.linear_mx(x, w, torch.empty(t, n, dtype=torch.bfloat16, device="cuda"))
+        want = stands_for(tail) @ stands_for(w).T
+        assert ((out[-last:].double() - want).abs() <= product_error(tail, w) + want.abs() * 2.0 ** -8).all()
+        assert not out[:-last].any()
+        del x, out
+    rows, h = 240000, 9216
+    stream, res = torch.zeros(rows, h, device="cuda"), torch.zeros(rows, h, dtype=torch.bfloat16, device="cuda")
+    stream[-last:], res[-last:] = rnd(last, h), rnd(last, h, seed=1)
+    y, w, before = o.MxRows.empty(rows, h), 1 + 0.1 * rnd(h, seed=2), stream[-last:].clone()
+    o.add_rmsnorm(stream, res, None, 0.0, w, 1e-6, y)
+    assert torch.equal(stream[-last:], before + res[-last:].float())
+    part = o.MxRows.empty(last, h)
+    o.rmsnorm(stream[-last:].contiguous(), w, 1e-6, part)
+    assert torch.equal(y.codes[-last:], part.codes) and not y.codes[:-last].any()
+
+
+@GPU
 def test_a_recorded_product_follows_its_inputs():
     o = ops()
     x, w = operands(2, 512, 1024)
