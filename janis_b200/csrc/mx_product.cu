@@ -383,6 +383,9 @@ __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, in
     if constexpr (EPI == EPI_NONE) {
         store_run<COLS>(v, o, t, n0, T, N, vec);
     } else {
+        // (a branch here also keeps the activation behind the arrival that gives tensor memory back: without one the compiler moves it in
+        // front, and 2,048 rows x 18,432 x 2,304 take 82 us instead of 75)
+        if (t >= T && (vec != 0 || o.codes != nullptr)) return;
         const int cols = N / 2, wide = o.codes != nullptr ? padded(cols) : cols, c = n0 / 2;
 #pragma unroll
         for (int u = 0; u < COLS / 16; ++u)
@@ -393,7 +396,6 @@ __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, in
             store_run<COLS / 2>(v, o, t, c, T, cols, vec);
             return;
         }
-        if (t >= T) return;
 #pragma unroll
         for (int g = 0; g < COLS / 64; ++g) {                         // (columns past the end are products with zeros)
             float big = 0.f;
