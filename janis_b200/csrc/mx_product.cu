@@ -58,6 +58,7 @@ constexpr int MAX_STAGES = 11;
 constexpr int FEW = 64;                        // rows of x at most
 constexpr int SCALE_BYTES = 2 * BLOCK_BYTES;   // of a stage: a block of W's, a block of x's
 constexpr int SCALE_COLS = 8;                  // of tensor memory
+constexpr int FEW_ROOM = 225 * 1024;           // of shared memory, beside what has a fixed place
 constexpr int few_smem(int stages, int NP, int split) {
     return stages * (A_BYTES + NP * 128 + SCALE_BYTES) + 1024 + (split > 1 ? NP * TILE * 4 : 0);
 }
@@ -83,7 +84,7 @@ __device__ __forceinline__ void store_rows(const float* sums, int rows, int row0
         }
         return;
     }
-    // a gate's up stands 8 rows behind it; for 8-bit rows a warp has the 32 columns of a group (SHARE is 64 at least)
+    // a gate's up stands 8 rows behind it; for 8-bit rows (SHARE is 64 at least) a warp has the 32 columns of a group
     constexpr int COLS = SHARE / 2;
     const int j = id % COLS, c = row0 / 2 + j, row = j / 8 * 16 + j % 8;
     const int all = N / 2, wide = o.codes != nullptr ? padded(all) : all;
@@ -122,16 +123,65 @@ __device__ __forceinline__ void store_rows(const float* sums, int rows, int row0
     }
 }
 
+// The same for 8-bit rows where a CTA's share is half (SPLIT 4) or a quarter (SPLIT 8) of the 64 rows of W behind a group: the CTAs of a group tell
+// each other their largest magnitudes, one for each row of x, counted in by `bar`.  False: they did not come.
+template <int SPLIT>
+__device__ __forceinline__ bool store_group_shares(const float* sums, float* largest, uint32_t bar, int rank, int rows, int row0, int N, const Out& o) {
+    constexpr int SHARE = TILE / SPLIT, COLS = SHARE / 2, STEP = 128 / COLS, CTAS = 32 / COLS, MOST = FEW / STEP;
+    const int id = threadIdx.x, j = id % COLS, c = row0 / 2 + j, row = j / 8 * 16 + j % 8, all = N / 2, wide = padded(all);
+    const int place = rank % CTAS, first = rank - place;
+    float v[MOST];
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+        const int m = id / COLS + u * STEP;
+        v[u] = 0.f;
+        if (m < rows && c < all) {
+            float gate = sums[m * SHARE + row], up = sums[m * SHARE + row + 8];
+#pragma unroll
+            for (int r = 1; r < SPLIT; ++r) {                         // in the order of the ranks
+                gate += sums[(r * rows + m) * SHARE + row];
+                up += sums[(r * rows + m) * SHARE + row + 8];
+            }
+            v[u] = gated(gate, up, o.epi, o);
+        }
+        float big = fabsf(v[u]);
+#pragma unroll
+        for (int s = COLS / 2; s > 0; s >>= 1) big = larger(big, __shfl_xor_sync(0xffffffffu, big, s));
+        if (m < rows && j < CTAS) {                                   // lane j tells CTA j of the group
+            const uint32_t at = (uint32_t)__cvta_generic_to_shared(largest + place * FEW + m);
+            asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];\n" ::"r"(in_cta(at, first + j)),
+                         "r"(__float_as_uint(big)), "r"(in_cta(bar, first + j))
+                         : "memory");
+        }
+    }
+    bool there = false;
+    for (int i = 0; i < 8 && !there; ++i) there = mbar_wait_cluster(bar, 0);
+    if (!__syncthreads_and(there ? 1 : 0)) return false;
+#pragma unroll
+    for (int u = 0; u < MOST; ++u) {
+        const int m = id / COLS + u * STEP;
+        if (m >= rows) break;
+        float big = largest[m];
+#pragma unroll
+        for (int p = 1; p < CTAS; ++p) big = larger(big, largest[p * FEW + m]);
+        const uint32_t byte = scale_byte_e4m3(big);
+        o.codes[(size_t)m * wide + c] = byte == 255u ? 0 : (uint8_t)two_e4m3(v[u] * inverse_scale(byte), 0.f);
+        if (c % GROUP == 0) o.scales[scale_at(m, c / BLOCK, wide / BLOCK) + c % BLOCK / GROUP] = (uint8_t)byte;
+    }
+    return true;
+}
+
 template <int SPLIT>
 __global__ void __launch_bounds__(128)
 few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const uint8_t* __restrict__ ws,
                 const uint8_t* __restrict__ xs, const Out o, int T, int N, int kp, int NP, int stages, int tmem_cols) {
     constexpr int SHARE = TILE / SPLIT;                              // rows of the tile that this CTA adds up and stores
     extern __shared__ unsigned char smem_raw[];
-    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 2];
+    __shared__ __align__(8) unsigned long long bars[2 * MAX_STAGES + 3];
     __shared__ uint32_t tmem_slot;
     __shared__ int failed, asked;                                     // asked: stages that copies were asked for
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ float largest[SPLIT > 2 ? SPLIT / 2 * FEW : 1];        // of a group of 8-bit rows, by the CTAs that share it
+    const int warp = threadIdx.x >> 5;
     const int rank = SPLIT > 1 ? (int)cg::this_cluster().block_rank() : 0;
     const int n0 = blockIdx.x / SPLIT * TILE;
     const int blocks = kp / BLOCK;
@@ -145,14 +195,17 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     float* sums = reinterpret_cast<float*>(smem_raw + (sums0 - raw));
     const uint32_t bar_full = (uint32_t)__cvta_generic_to_shared(bars);
     const uint32_t bar_empty = bar_full + 8 * MAX_STAGES, bar_done = bar_full + 16 * MAX_STAGES, bar_sums = bar_done + 8;
+    const uint32_t bar_largest = bar_sums + 8;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
         mbar_init(bar_done, 1);
         mbar_init(bar_sums, 1);
+        mbar_init(bar_largest, 1);
         failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         if (SPLIT > 1) mbar_expect_tx(bar_sums, T * TILE * 4);
+        if (SPLIT > 2) mbar_expect_tx(bar_largest, SPLIT / 2 * T * 4);
     }
     if (warp == 0) tmem_alloc((uint32_t)__cvta_generic_to_shared(&tmem_slot), tmem_cols);
     fence_before_sync();
@@ -259,10 +312,14 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     }
     ok = __syncthreads_and(ok ? 1 : 0);
     if (warp == 0) tmem_free(tmem, tmem_cols);
-    if (!ok) {
-        if (threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
-        return;
+    if (!ok && threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
+    if constexpr (SPLIT > 2) {
+        if (o.codes != nullptr) {                                     // (a CTA that gave up stays for what the others tell it)
+            if (!store_group_shares<SPLIT>(sums, largest, bar_largest, rank, T, n0 + rank * SHARE, N, o) && threadIdx.x == 0) atomicAdd(&g_timeouts, 1);
+            return;
+        }
     }
+    if (!ok) return;
     store_rows<SPLIT>(sums, T, n0 + rank * SHARE, N, o);
 }
 
@@ -883,18 +940,17 @@ static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, con
     const int NP = (T + 15) / 16 * 16;
     // (8-bit rows are padded to whole blocks of 128 columns: 256 rows of gates and ups)
     const int tiles = o.codes != nullptr ? padded(N / 2) / (TILE / 2) : (N + TILE - 1) / TILE, blocks = kp / BLOCK;
-    const int most_split = o.codes != nullptr ? 2 : 8;                // (a group of 8-bit rows lies within a CTA's share)
     if (split == 0) {
         // K is shared while all CTAs are resident, two an SM, and keep four blocks each.  A cluster lies within a GPC, of whose 16 to 18
         // SMs four clusters of 8 take all: 32 in all, or 48 of three CTAs an SM, which pay where K is long only.  One row, us with 1, 2, 4,
         // 8 CTAs: 2,304 x 2,048 5.3, 3.6, 2.9, 3.3; 4,096 x 2,304 5.8, 3.8, 3.4, 4.2; 2,304 x 9,216 18, 10, 6.4, 4.8; 18,432 x 2,304 7.2, 6.1;
         // 4,608 x 4,096 -, -, 4.4, 4.8 (36 tiles); 4,608 x 36,864 66, 34, 22, 20 (36 tiles).
         split = 1;
-        while (split < most_split && tiles * split * 2 <= 2 * sm_count() && blocks >= split * 2 * 4 && (split < 4 || tiles <= 32)) split *= 2;
-        if (split == 4 && most_split == 8 && NP <= 32 && tiles > 32 && tiles <= 48 && blocks >= 128) split = 8;
+        while (split < 8 && tiles * split * 2 <= 2 * sm_count() && blocks >= split * 2 * 4 && (split < 4 || tiles <= 32)) split *= 2;
+        if (split == 4 && NP <= 32 && tiles > 32 && tiles <= 48 && blocks >= 128) split = 8;
     }
-    if (split > most_split || split > blocks || (split & (split - 1)) != 0) return fail("mx_product: a split of %d is not possible here", split);
-    const int most = 227 * 1024 - 512;
+    if (split > 8 || split > blocks || (split & (split - 1)) != 0) return fail("mx_product: a split of %d is not possible here", split);
+    const int most = FEW_ROOM;
     if (stages == 0) {
         // a ring as deep as the SM's memory allows for the CTAs that share it
         const int room = split == 8 && NP <= 32 && tiles > 32 ? 74 * 1024 : split > 1 || tiles > sm_count() ? 113 * 1024 : most;
@@ -916,7 +972,7 @@ static int few_rows(const uint8_t* xc, const uint8_t* xs, const uint8_t* wc, con
     static cudaError_t e = cudaSuccess;
     std::call_once(once, [] {
         for (const auto k : {few_rows_kernel<1>, few_rows_kernel<2>, few_rows_kernel<4>, few_rows_kernel<8>})
-            if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 512);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_ROOM);
     });
     if (e != cudaSuccess) return fail("mx_product: shared memory refused: %s", cudaGetErrorString(e));
     return launch_kernel("mx_product", kernel, dim3(tiles * split), dim3(128), few_smem(stages, NP, split), stream, split, mw, mx, ws, xs, o,

@@ -349,7 +349,7 @@ def test_any_split_and_any_depth_of_the_ring(t, n, k):
 
 
 @GPU
-@pytest.mark.parametrize("kernel,split", [(1, 0), (2, 0), (3, 0), (4, 2), (4, 4), (4, 8)])
+@pytest.mark.parametrize("kernel,split", [(1, 0), (1, 4), (1, 8), (2, 0), (3, 0), (4, 2), (4, 4), (4, 8)])
 @pytest.mark.parametrize("t,n,k", [(1, 144, 1024), (40, 1008, 1100), (129, 128, 2048), (260, 400, 1280), (33, 48016, 1030), (150, 333, 1100)])
 def test_every_kernel_takes_every_size(t, n, k, kernel, split):
     o = ops()
@@ -364,7 +364,7 @@ def test_every_kernel_takes_every_size(t, n, k, kernel, split):
         assert ((got[0].double() - want).abs() <= tol).all()
         half = o.linear_mx(x, w, torch.empty(t, n, dtype=torch.bfloat16, device="cuda"))
         assert torch.equal(half, got[0].bfloat16())
-        if n % 16 == 0 and split < 8:
+        if n % 16 == 0 and (split < 8 or kernel == 1):
             for epi in (1, 3):
                 v = o.linear_mx(x, w, torch.full((t, n // 2), NAN, device="cuda"), epi)
                 rows, again = o.MxRows.empty(t, n // 2), o.MxRows.empty(t, n // 2)
