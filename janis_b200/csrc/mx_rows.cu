@@ -1,7 +1,5 @@
 // Rows in and out of the 8-bit microscaling form (mx.cuh): the norms and the gated activation that leave it for the products
 // behind them, plain rows, the weights' 4-bit form at load, and the values that either form stands for.
-#include <limits.h>
-
 #include "mx.cuh"
 
 namespace janis {
@@ -394,7 +392,7 @@ JANIS_EXPORT int janis_mx_norm_rows(const void* block) {
     const float eps_post = (float)a.eps_post, eps_next = (float)a.eps_next;
     const int* rows = a.rows;
     uint8_t *codes = a.codes, *scales = a.scales;
-    if (a.R > INT_MAX || a.H > INT_MAX) return fail("mx_norm_rows: sizes pass 2^31");
+    if (a.R > 1 << 30 || a.H > 1 << 30) return fail("mx_norm_rows: sizes pass 2^30");
     const int res_dtype = (int)a.res_dtype, n_part = (int)a.n_part, R = (int)a.R, H = (int)a.H;
     const long long part_stride = a.part_stride;
     cudaStream_t stream = a.stream;

@@ -81,6 +81,19 @@ __device__ __forceinline__ void tmem_load32(uint32_t* r, uint32_t addr) {
         : "r"(addr));
 }
 
+// A load of what no CTA reads again in this kernel: first to leave L2, where others' lines may stay.
+__device__ __forceinline__ uint64_t read_once() {
+    uint64_t p;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;\n" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void load_2d_by(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3}], [%4], %5;\n" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar), "l"(policy)
+        : "memory");
+}
+
 // ---- two CTAs of a cluster as one: the tensor cores of both SMs take one product of 256 rows, half of them (and half of the other operand's rows)
 // in the shared memory of each; one thread of the first CTA issues for both.
 __device__ __forceinline__ void pair_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {      // bar: in either CTA
