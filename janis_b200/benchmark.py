@@ -856,6 +856,33 @@ def compare(sizes=("gemma2-2b", "gemma2-9b", "gemma2-27b"), layers: int = 4, pre
     return rec
 
 
+def compare_weights(sizes=("gemma2-2b", "gemma2-27b"), layers: int | None = None, batches=(1, 8, 64), prompts=(128, 512, 2048, 8192),
+                    length: int = 1024, steps: int = 64, warmup: int = 8) -> dict:
+    """Gemma2 with its layers' matrices in 4 bits beside bfloat16, random weights: decode steps of several batches (sequences of `length`
+    tokens), prompt steps, and the device memory that weights and cache take."""
+    import janis_b200
+    rec = {"compare": "mx4 weights beside bfloat16", "data": "synthetic", "length": length, "steps": steps, "sizes": {}}
+    for name in sizes:
+        raw = load_config(name)
+        if layers:
+            raw = dict(raw, num_hidden_layers=layers)
+            raw.pop("layer_types", None)
+        rec["sizes"][name] = out = {}
+        for weights in (None, "mx4"):
+            before = torch.cuda.memory_allocated()
+            eng = janis_b200.from_config(raw, seed=0, dtype="bfloat16", max_tokens=max(max(batches) * (length + steps + warmup + 64), max(prompts) + 64),
+                                         max_batch=max(batches), max_context=max(max(prompts), length + steps + warmup), weights=weights)
+            held = torch.cuda.memory_allocated() - before
+            out[weights or "bf16"] = {
+                "memory_gib": round(held / 2 ** 30, 1),
+                "decode_ms_per_step": {b: round(measure_decode(eng, [length] * b, steps, warmup, runs=3)["ms_per_step"], 4) for b in batches},
+                "prompt_ms": {n: round(measure_prefill(eng, n)["ms"], 3) for n in prompts}}
+            eng.close()
+            del eng
+            torch.cuda.empty_cache()
+    return rec
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(prog="janis bench")
     ap.add_argument("--gpus", type=int, default=1)
@@ -877,7 +904,7 @@ def main(argv=None) -> int:
                     "instead of sequences that all reach --context")
     ap.add_argument("--profile", choices=["decode", "prefill"], default="",
                     help="open the CUDA profiler range around two timed decode steps, or the last prompt step")
-    ap.add_argument("--compare", choices=["sigalorn", "nosolix", "vivazen", "dekutar", "larulorn", "mugedra"], default="",
+    ap.add_argument("--compare", choices=["sigalorn", "nosolix", "vivazen", "dekutar", "larulorn", "mugedra", "mx4"], default="",
                     help="instead of the benchmark: Sigalorn beside Gemma2, Nosolix, Vivazen or Dekutar beside Sigalorn, or Larulorn or Mugedra "
                     "beside Nosolix, at equal layer sizes (prompt and decode throughput, and each design's own kernels against their rooflines); "
                     "--config picks one size")
@@ -889,6 +916,10 @@ def main(argv=None) -> int:
     if a.gpus != 1:
         print(f"janis_b200 is a one-GPU library: --gpus {a.gpus} is not supported")
         return 2
+    if a.compare == "mx4":
+        sizes = ("gemma2-2b", "gemma2-27b") if "--config" not in (argv or sys.argv) else ((a.config if a.config.startswith("gemma2-") else "gemma2-" + a.config),)
+        print(json.dumps(compare_weights(sizes, a.layers or None)))
+        return 0
     if a.compare:
         sizes = ("gemma2-2b", "gemma2-9b", "gemma2-27b") if a.config == "gemma2-2b" and "--config" not in (argv or sys.argv) \
             else ((a.config if a.config.startswith("gemma2-") else "gemma2-" + a.config),)

@@ -1,5 +1,7 @@
 // Rows in and out of the 8-bit microscaling form (mx.cuh): the norms and the gated activation that leave it for the products
 // behind them, plain rows, the weights' 4-bit form at load, and the values that either form stands for.
+#include <type_traits>
+
 #include "mx.cuh"
 
 namespace janis {
@@ -61,8 +63,31 @@ norm_rows_kernel(float* __restrict__ h, const TR* __restrict__ res, int n_part, 
         store_group(i < H ? hr[i] * inv * w_next[i] : 0.f, codes, scales, r, i / GROUP, kp / GROUP, kp);
 }
 
+// Sum over a block in a fixed order, the warps' sums in 64 bits: a row's factor then has little more of rounding than its lanes' sums, which
+// are many and err at random.  `scratch` holds at least 32.
+__device__ __forceinline__ double block_sum_long(float v, float* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarp = (blockDim.x + 31) >> 5;
+    v = warp_sum(v);
+    if (nwarp == 1) return v;
+    __syncthreads();            // scratch may still be read from an earlier call
+    if (lane == 0) scratch[warp] = v;
+    __syncthreads();
+    double t = 0.;
+    for (int w = 0; w < nwarp; ++w) t += (double)scratch[w];
+    return t;
+}
+
+// 1 / sqrt(mean) in 64 bits from the float `f`: one step of Newton's, whose error is the square of f's
+__device__ __forceinline__ double refined(float f, double mean) { return fma(0.5 * f, fma(-mean * f, (double)f, 1.0), (double)f); }
+
+struct Nothing {};                 // for values that are what they are
+
 // Eight values a thread, four threads a group, sixteen a block of 128: codes as 8 bytes, the block's four scales as 4.  Whole warps call it.
-__device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* codes, uint8_t* scales, int r, int j, int blocks, bool live) {
+// With `exact` (value e in 64 bits) a value within 8 units in the last place of the middle between two codes, which a float's roundings may turn, is
+// formed again and rounded once: one value in 60,000, for three instructions a value.
+template <typename F>
+__device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* codes, uint8_t* scales, int r, int j, int blocks, bool live,
+                                                     F exact) {
     float big = fabsf(v[0]);
 #pragma unroll
     for (int e = 1; e < 8; ++e) big = larger(big, v[e]);
@@ -73,9 +98,30 @@ __device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* co
     uint32_t four = byte << (8 * (threadIdx.x >> 2 & 3));
     four |= __shfl_xor_sync(0xffffffffu, four, 4);
     four |= __shfl_xor_sync(0xffffffffu, four, 8);
+    float x[8];
+    bool near = false;
+    // (the last 20 bits of a float are what a code with 3 bits behind the point leaves; codes below the normal ones are not looked at)
+    const auto near_middle = [](float a) { return ((__float_as_uint(a) + 0x80008u) & 0xfffffu) <= 0x10u; };
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        x[e] = v[e] * inv;
+        near = near || near_middle(x[e]);
+    }
+    if constexpr (!std::is_same<F, Nothing>::value) {
+        if (near && byte != 255u && live) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (!near_middle(x[e])) continue;                     // (nor are the zeros behind a row's end)
+                const double y = exact(e) * (double)inv;
+                float f = __double2float_rz(y);                       // rounded to odd, so that rounding it again is rounding y once
+                if ((double)f != y) f = __uint_as_float(__float_as_uint(f) | 1u);
+                x[e] = f;
+            }
+        }
+    }
     uint2 q;
-    q.x = two_e4m3(v[0] * inv, v[1] * inv) | two_e4m3(v[2] * inv, v[3] * inv) << 16;
-    q.y = two_e4m3(v[4] * inv, v[5] * inv) | two_e4m3(v[6] * inv, v[7] * inv) << 16;
+    q.x = two_e4m3(x[0], x[1]) | two_e4m3(x[2], x[3]) << 16;
+    q.y = two_e4m3(x[4], x[5]) | two_e4m3(x[6], x[7]) << 16;
     if (byte == 255u) q = make_uint2(0u, 0u);
     if (!live) return;
     *reinterpret_cast<uint2*>(codes + ((size_t)r * blocks * BLOCK + (size_t)j * 8)) = q;
@@ -89,7 +135,7 @@ template <typename TR, int VPT>
 __global__ void __launch_bounds__(640)
 norm_rows_odd_kernel(float* __restrict__ h, const TR* __restrict__ res, const float* __restrict__ w_post, float eps_post,
                      const float* __restrict__ w_next, float eps_next, const int* __restrict__ rows, uint8_t* __restrict__ codes,
-                     uint8_t* __restrict__ scales, int H) {
+                     uint8_t* __restrict__ scales, int H, double share) {
     extern __shared__ __align__(16) float y[];                        // the row, on its way from a value a lane to pieces of 8
     __shared__ float scratch[32];
     const int r = blockIdx.x, kp = padded(H);
@@ -103,27 +149,36 @@ norm_rows_odd_kernel(float* __restrict__ h, const TR* __restrict__ res, const fl
         hv[k] = i < H ? hr[i] : 0.f;
         v[k] = res != nullptr && i < H ? to_float(res[(size_t)r * H + i]) : 0.f;
     }
+    double mean_post = 1.;
+    float post = 1.f;
     if (res != nullptr) {
-        float inv = 1.f;
         if (w_post != nullptr) {
 #pragma unroll
             for (int k = 0; k < VPT; ++k) ss = fmaf(v[k], v[k], ss);
-            ss = block_sum(ss, scratch);
-            inv = 1.0f / sqrtf(ss / (float)H + eps_post);
+            mean_post = fma(block_sum_long(ss, scratch), share, (double)eps_post);
+            post = 1.0f / sqrtf((float)mean_post);
             ss = 0.f;
         }
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int i = threadIdx.x + k * blockDim.x;
             if (i >= H) continue;
-            hv[k] += w_post != nullptr ? v[k] * inv * w_post[i] : v[k];
-            hr[i] = hv[k];
+            hv[k] += w_post != nullptr ? v[k] * post * w_post[i] : v[k];
         }
     }
 #pragma unroll
     for (int k = 0; k < VPT; ++k) ss = fmaf(hv[k], hv[k], ss);
-    ss = block_sum(ss, scratch);
-    const float inv = 1.0f / sqrtf(ss / (float)H + eps_next);
+    const double mean = fma(block_sum_long(ss, scratch), share, (double)eps_next);
+    const float inv = 1.0f / sqrtf((float)mean);
+    // (the sum as it was before it was rounded: what it is made of is still there)
+    const auto exact = [&](int i) {
+        double t = hr[i];
+        if (res != nullptr) {
+            const double add = to_float(res[(size_t)r * H + i]);
+            t += w_post != nullptr ? add * refined(post, mean_post) * (double)w_post[i] : add;
+        }
+        return t * (double)w_next[i] * refined(inv, mean);
+    };
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int i = threadIdx.x + k * blockDim.x;
@@ -133,7 +188,14 @@ norm_rows_odd_kernel(float* __restrict__ h, const TR* __restrict__ res, const fl
     for (int j = threadIdx.x; j - (int)(threadIdx.x & 31) < kp / 8; j += blockDim.x) {      // whole warps
         float e[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (j < kp / 8) load_eight(y + j * 8, e);
-        store_eight_of_group(e, codes, scales, r, j, kp / BLOCK, j < kp / 8);
+        store_eight_of_group(e, codes, scales, r, j, kp / BLOCK, j < kp / 8, [&](int at) { return exact(j * 8 + at); });
+    }
+    if (res == nullptr) return;
+    __syncthreads();                                                  // (what is exact reads the stream as it was)
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i < H) hr[i] = hv[k];
     }
 }
 
@@ -156,15 +218,18 @@ template <> struct Eight<float> {
 // The same with the row in registers: thread i takes the pieces of 8 values i, i + blockDim, ... (H a multiple of 8, at most VPT of them), so that
 // each input is read once, 16 bytes at a time, and a row's scales leave four at a time.  Bound by memory at many rows, where what counts is how
 // many rows an SM has on its way: the residual stays as it is stored, the norms' weights are read where they are used, and a thread takes two
-// pieces.  8,192 rows of 2,304: 43.2 us with one piece a thread, 37.9 with two, 40.3 with five, 59.8 with nine (a warp a row); 31.9 at the copy's
-// bandwidth.  Held weights and eight floats of the residual a thread: 60.0; rows that the copy engine brings into a ring: 66.7.  At few rows,
-// bound by latency, one piece: one row 2.4 us, with two 2.8.
+// pieces.  8,192 rows of 2,304, in us: one piece a thread 43.2, two 37.9, five 40.3, nine (a warp a row) 59.8; 31.9 at the copy's bandwidth.
+// With the warps' sums in 64 bits and values near a middle formed again 40.7, for half as many codes that differ from those of 64 bits (69 of 75
+// million; plain float arithmetic 144).  Held weights and eight floats of the residual a thread: 60.0; rows that the copy engine brings into a
+// ring: 66.7.  At few rows, bound by latency, one piece: one row 2.5 us, with two 2.8.
 template <typename TR, int VPT>
-__global__ void __launch_bounds__(640)
+__global__ void __launch_bounds__(640, VPT == 3 ? 1 : 2)      // (48 registers at most: what is rare takes more otherwise)
 norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, const float* __restrict__ w_post, float eps_post,
                       const float* __restrict__ w_next, float eps_next, const int* __restrict__ rows, uint8_t* __restrict__ codes,
-                      uint8_t* __restrict__ scales, int H) {
+                      uint8_t* __restrict__ scales, int H, double share) {
     __shared__ float scratch[32];
+    // (few rows, which want to be quick, have few values that lie near a middle)
+    const auto row_sum = [&](float v) { return VPT == 1 ? (double)block_sum(v, scratch) : block_sum_long(v, scratch); };
     const int r = blockIdx.x, pieces = H / 8, all = padded(H) / 8;
     grid_dependents_launch();
     grid_dependency_wait();
@@ -183,16 +248,17 @@ norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, const fl
         }
     }
     float ss = 0.f;
+    double mean_post = 1.;
+    float post = 1.f;
     if (res != nullptr) {
-        float inv = 1.f;
         if (w_post != nullptr) {
 #pragma unroll
             for (int k = 0; k < VPT; ++k)
                 if ((int)threadIdx.x + k * (int)blockDim.x < pieces)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ss = fmaf(v[k].get(e), v[k].get(e), ss);
-            ss = block_sum(ss, scratch);
-            inv = 1.0f / sqrtf(ss / (float)H + eps_post);
+            mean_post = fma(row_sum(ss), share, (double)eps_post);
+            post = 1.0f / sqrtf((float)mean_post);
             ss = 0.f;
         }
 #pragma unroll
@@ -203,20 +269,28 @@ norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, const fl
                 float w[8];
                 load_eight(w_post + j * 8, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) hv[k][e] += v[k].get(e) * inv * w[e];
+                for (int e = 0; e < 8; ++e) hv[k][e] += v[k].get(e) * post * w[e];
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) hv[k][e] += v[k].get(e);
             }
-            store_eight(hr + j * 8, hv[k]);
         }
     }
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(hv[k][e], hv[k][e], ss);
-    ss = block_sum(ss, scratch);
-    const float inv = 1.0f / sqrtf(ss / (float)H + eps_next);
+    const double mean = fma(row_sum(ss), share, (double)eps_next);
+    const float inv = 1.0f / sqrtf((float)mean);
+    // (the sum as it was before it was rounded: what it is made of is still there)
+    const auto exact = [&](int i) {
+        double t = hr[i];
+        if (res != nullptr) {
+            const double add = to_float(res[(size_t)r * H + i]);
+            t += w_post != nullptr ? add * refined(post, mean_post) * (double)w_post[i] : add;
+        }
+        return t * (double)w_next[i] * refined(inv, mean);
+    };
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
         const int j = threadIdx.x + k * blockDim.x;
@@ -226,8 +300,9 @@ norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, const fl
         for (int e = 0; e < 8; ++e) w[e] = 0.f;
         if (j < pieces) load_eight(w_next + j * 8, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) hv[k][e] = hv[k][e] * inv * w[e];
-        store_eight_of_group(hv[k], codes, scales, r, j, all / 16, j < all);
+        for (int e = 0; e < 8; ++e) w[e] = hv[k][e] * inv * w[e];
+        store_eight_of_group(w, codes, scales, r, j, all / 16, j < all, [&](int at) { return exact(j * 8 + at); });
+        if (res != nullptr && j < pieces) store_eight(hr + j * 8, hv[k]);
     }
 }
 
@@ -284,7 +359,7 @@ plain_rows_vec_kernel(const T* __restrict__ x, int act, float limit, float alpha
                     v[e] = act == 2 ? clamped_gate(g[e], u[e], limit, alpha, up_add) : (act == 0 ? gelu_tanh(g[e]) : g[e] / (1.0f + expf(-g[e]))) * u[e];
             }
         }
-        store_eight_of_group(v, codes, scales, r, j, kp / BLOCK, live);
+        store_eight_of_group(v, codes, scales, r, j, kp / BLOCK, live, Nothing());
     }
 }
 
@@ -332,7 +407,8 @@ static int norm_rows(float* h, const TR* res, int n_part, size_t part_stride, co
     if (!vec && n_part <= 1 && pieces <= 640) {
         const int n = pieces > 320 || (R >= 768 && pieces > 80) ? 8 : 4;
         return launch_kernel("mx_norm_rows", n == 4 ? norm_rows_odd_kernel<TR, 4> : norm_rows_odd_kernel<TR, 8>, dim3(R),
-                             dim3((pieces * 8 / n + 31) / 32 * 32), pieces * 32, stream, 1, h, res, w_post, eps_post, w_next, eps_next, rows, codes, scales, H);
+                             dim3((pieces * 8 / n + 31) / 32 * 32), pieces * 32, stream, 1, h, res, w_post, eps_post, w_next, eps_next, rows, codes, scales, H,
+                             1.0 / H);
     }
     if (!vec || n_part > 1 || pieces > 1920)
         return launch_kernel("mx_norm_rows", norm_rows_kernel<TR>, dim3(R), dim3(256), 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post,
@@ -340,7 +416,7 @@ static int norm_rows(float* h, const TR* res, int n_part, size_t part_stride, co
     const int vpt = pieces > 1280 ? 3 : pieces > 640 || (R >= 768 && pieces > 160) ? 2 : 1;
     const auto kernel = vpt == 1 ? norm_rows_vec_kernel<TR, 1> : vpt == 2 ? norm_rows_vec_kernel<TR, 2> : norm_rows_vec_kernel<TR, 3>;
     return launch_kernel("mx_norm_rows", kernel, dim3(R), dim3(((pieces + vpt - 1) / vpt + 31) / 32 * 32), 0, stream, 1, h, res, w_post, eps_post,
-                         w_next, eps_next, rows, codes, scales, H);
+                         w_next, eps_next, rows, codes, scales, H, 1.0 / H);      // (share: a mean is a sum times 1 / H)
 }
 
 static int blocks_for(size_t warps) {
