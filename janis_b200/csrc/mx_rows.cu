@@ -129,8 +129,10 @@ __device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* co
 }
 
 // The same with the row in registers where rows start anywhere or are no whole pieces of 8: thread i takes the values i, i + blockDim, ... (VPT of
-// them), 4 or 2 bytes at a time, and the row is turned to pieces of 8 in shared memory.  8,192 rows of 1,001: 33.8 us with 8 values a
-// thread, 37.2 with 4, 45.3 with a value a lane to the end; of 2,303 107, whatever a thread takes (loads and stores of single values).
+// them), 4 or 2 bytes at a time, and the row is turned to pieces of 8 in shared memory.  8,192 rows of 1,001: 36.0 us with 8 values a
+// thread; of 2,303 98 (loads and stores of single values).  Rows above 4,096 leave room for one block of 8 values a thread on an SM (64
+// registers, 513 threads or more): with 16 there are two, 2,048 rows of 4,607 62.9 us against 82.1, 256 10.0 against 12.5; a single row, which
+// has the SM to itself, 6.6 against 5.3.  Rows brought in 16-byte pieces through shared memory: 41.6 us (of 1,001), 105 (of 2,303), 62.8 (of 4,607).
 template <typename TR, int VPT>
 __global__ void __launch_bounds__(640)
 norm_rows_odd_kernel(float* __restrict__ h, const TR* __restrict__ res, const float* __restrict__ w_post, float eps_post,
@@ -405,10 +407,10 @@ static int norm_rows(float* h, const TR* res, int n_part, size_t part_stride, co
     const bool vec = H % 8 == 0 && (((uintptr_t)h | (uintptr_t)res | (uintptr_t)w_post | (uintptr_t)w_next) & 15) == 0 && part_stride % 8 == 0;
     const int pieces = padded(H) / 8;
     if (!vec && n_part <= 1 && pieces <= 640) {
-        const int n = pieces > 320 || (R >= 768 && pieces > 80) ? 8 : 4;
-        return launch_kernel("mx_norm_rows", n == 4 ? norm_rows_odd_kernel<TR, 4> : norm_rows_odd_kernel<TR, 8>, dim3(R),
-                             dim3((pieces * 8 / n + 31) / 32 * 32), pieces * 32, stream, 1, h, res, w_post, eps_post, w_next, eps_next, rows, codes, scales, H,
-                             1.0 / H);
+        const int n = pieces > 512 && R > 148 ? 16 : pieces > 320 || (R >= 768 && pieces > 80) ? 8 : 4;
+        const auto kernel = n == 4 ? norm_rows_odd_kernel<TR, 4> : n == 8 ? norm_rows_odd_kernel<TR, 8> : norm_rows_odd_kernel<TR, 16>;
+        return launch_kernel("mx_norm_rows", kernel, dim3(R), dim3((pieces * 8 / n + 31) / 32 * 32), pieces * 32, stream, 1, h, res, w_post, eps_post, w_next,
+                             eps_next, rows, codes, scales, H, 1.0 / H);
     }
     if (!vec || n_part > 1 || pieces > 1920)
         return launch_kernel("mx_norm_rows", norm_rows_kernel<TR>, dim3(R), dim3(256), 0, stream, 1, h, res, n_part, part_stride, w_post, eps_post,

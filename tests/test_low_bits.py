@@ -172,7 +172,8 @@ def norm_error(h):
 @GPU
 @pytest.mark.parametrize("post", [True, False])
 @pytest.mark.parametrize("res", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,h", [(1, 8), (1, 2304), (3, 33), (5, 4608), (130, 1000), (64, 36), (2, 9216), (2, 20000)])
+@pytest.mark.parametrize("rows,h", [(1, 8), (1, 2304), (3, 33), (5, 4608), (130, 1000), (64, 36), (2, 9216), (2, 20000), (160, 4607),
+                                    (800, 1001)])
 def test_norm_with_the_residuals_addition(rows, h, res, post):
     o = ops()
     x, r = rnd(rows, h, seed=1) * torch.exp(rnd(h, seed=2)), (rnd(rows, h, seed=3) * 2).to(res)
