@@ -215,7 +215,7 @@ few_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 
     // this CTA's share of K: value blocks rank, rank + SPLIT, ...
     const int nk = (blocks - rank + SPLIT - 1) / SPLIT;
-    // (a tile past W's rows, which only makes the padding of 8-bit rows, finds zeros there whatever their scales)
+    // (a tile past W's rows, which only makes the padding of 8-bit rows, finds zeros there; their scales mean nothing, and its columns count as 0)
     const uint8_t* w_scales = ws + (size_t)min(n0 / BLOCK, (N - 1) / BLOCK) * blocks * BLOCK_BYTES;
 
     grid_dependents_launch();
@@ -435,6 +435,15 @@ __device__ __forceinline__ void store_run(uint32_t* v, const Out& o, int t, int 
     }
 }
 
+// 8-bit rows are padded with zeros of scale 1: columns from `left` on count as 0, whatever is there.  Behind W's rows the copies find zeros, but the
+// scales that fill their block of 128 mean nothing, and a zero under a scale of NaN is a NaN.  (Whole warps agree on `left`; only the last tiles enter.)
+template <int COUNT>
+__device__ __forceinline__ void no_columns_from(uint32_t* v, int left) {
+    if (left >= COUNT) return;
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) v[j] = j < left ? v[j] : 0u;
+}
+
 // The end of a row's run of COLS columns of sums from column n0 on (rows of W), by the thread that holds them; a whole warp calls it.
 template <int COLS, int EPI>
 __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, int t, int n0, int T, int N, int vec) {
@@ -454,8 +463,9 @@ __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, in
             store_run<COLS / 2>(v, o, t, c, T, cols, vec);
             return;
         }
+        no_columns_from<COLS / 2>(v, cols - c);
 #pragma unroll
-        for (int g = 0; g < COLS / 64; ++g) {                         // (columns past the end are products with zeros)
+        for (int g = 0; g < COLS / 64; ++g) {
             float big = 0.f;
 #pragma unroll
             for (int j = 0; j < 32; ++j) big = larger(big, __uint_as_float(v[g * 32 + j]));
@@ -509,7 +519,7 @@ many_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constan
 
     if (warp == 0 && elect_one()) {
         const int w_last = (N - 1) / BLOCK;
-        const auto load_w = [&](int s, int kb, int n) {               // (what is past W's rows is zeros whatever their scales)
+        const auto load_w = [&](int s, int kb, int n) {               // (past W's rows are zeros, whose scales mean nothing: such columns count as 0)
             mbar_expect_tx(bar_full + 8 * s, X_BYTES + A_PACKED + 2 * BLOCK_BYTES);
             tma_load_2d(stage0 + s * MANY_STAGE + X_BYTES, &map_w, kb * BLOCK, n * 128, bar_full + 8 * s);
             bulk_load(scales0 + s * MANY_SCALES + BLOCK_BYTES, ws + ((size_t)min(n, w_last) * blocks + kb) * BLOCK_BYTES, BLOCK_BYTES, bar_full + 8 * s);
@@ -904,6 +914,7 @@ shared_rows_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
             return;
         }
         constexpr int HELD = RUN / 2, RUNS = 32 / HELD;               // columns of a thread: 16 or 8 of a group of 32, the others in other warps
+        no_columns_from<HELD>(v, cols - c);
         float big = 0.f;
 #pragma unroll
         for (int j = 0; j < HELD; ++j) big = larger(big, __uint_as_float(v[j]));
