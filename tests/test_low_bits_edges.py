@@ -79,3 +79,94 @@ def test_a_product_behind_a_cut_weight_is_finite(t):
     o.linear_mx(x, o.mx_weight(gate_up)[:144], act, o.EPI_GATED_GELU)
     out = o.linear_mx(act, down, torch.empty(t, 40, device="cuda"))
     assert torch.isfinite(out).all()
+
+
+# ---------------------------------------------------------------------------
+# next to the middle between two codes
+# ---------------------------------------------------------------------------
+
+def near_middles(rows, h, most, eps=0.0, seed=0):
+    """(stream [rows, h], w_next, y in 64 bits, whether a place counts): whole numbers up to `most` whose signs alone differ from row to row, and
+    weights that bring every value to within half a unit in its last place (2^-24 of it) of the middle between two codes of scale 1; the first
+    value of a group of 32 keeps its scale there.  Sums of squares are whole numbers, so the mean is known exactly."""
+    g = torch.Generator().manual_seed(seed)
+    base = torch.randint(1, most + 1, (h,), generator=g).double()
+    if (base * base).sum() % 2 == 0:                       # an odd sum: what passes 2^24 is no float
+        base[0] += 1 if base[0] < most else -1
+    sign = torch.randint(0, 2, (rows, h), generator=g).double() * 2 - 1
+    middle = (1 + (2 * torch.randint(0, 8, (h,), generator=g) + 1) / 16) * 2.0 ** torch.randint(-6, 8, (h,), generator=g)
+    middle[::32] = 390.0
+    w = (middle.double() * torch.sqrt((base * base).mean() + eps) / base).float()
+    return (base * sign).float(), w, middle
+
+
+def codes_of(h, w, eps):
+    """Codes' values of the norm in 64 bits, and y."""
+    h = h.double()
+    y = h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps) * w.double()
+    return R.quantised(y, *E4M3)[1], y
+
+
+def check_middles(out, stream, w, middle, eps, what):
+    """Codes are those of the value rounded once.  What is left out lies within 2^-28 of a middle: the path in 64 bits is
+    exact to 2^-45, and what is below the stream's roundings changes the mean by less than 2^-28 (looked at here), half of which goes
+    into a root."""
+    want, y = codes_of(stream.cpu(), w.cpu(), eps)
+    rows, h = y.shape
+    held = stream.cpu().float().double()
+    assert (((held * held).mean(-1) / (stream.cpu().double() ** 2).mean(-1) - 1).abs() < 2.0 ** -28).all()
+    sure = torch.ones_like(want, dtype=torch.bool)
+    sure[:, :h] = (y.abs() / middle - 1).abs() > 2.0 ** -28
+    got = code_values(out).cpu()
+    assert (scale_rows(out)[:, :-(-h // 32)] == 127).all(), f"{what}: scales"
+    bad = (got != want) & sure
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {int(sure.sum())} codes are not those of the value rounded once, first at {bad.nonzero()[0].tolist()}"
+
+
+@pytest.mark.parametrize("h", [1001, 2304])
+def test_floats_alone_turn_planted_codes(h):
+    """(So the tests below see whether the second look is there.)"""
+    stream, w, middle = near_middles(3, h, 7)
+    want, y = codes_of(stream, w, 0.0)
+    assert ((y.abs() / middle - 1).abs()[:, 1:] < 2.0 ** -23).float().mean() > 0.9
+    plain = stream * (1.0 / torch.sqrt((stream * stream).mean(-1, keepdim=True))) * w
+    turned = (R.quantised(plain.double(), *E4M3)[1] != want).float().mean()
+    assert turned > 0.1
+
+
+# eight values a thread and one, two, three pieces; four, eight, sixteen values a thread where rows start anywhere
+NORMS = [(3, 1024), (2, 2304), (800, 2304), (5, 4608), (3, 8200), (2, 12288), (5, 1001), (800, 1001), (160, 4607), (3, 33)]
+
+
+@GPU
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -10])
+@pytest.mark.parametrize("rows,h", NORMS)
+def test_norms_round_once_next_to_a_middle(rows, h, eps):
+    o = ops()
+    stream, w, middle = near_middles(rows, h, 7, eps, seed=h)
+    out, x = o.MxRows.empty(rows, h), stream.cuda()
+    o.rmsnorm(x, w.cuda(), eps, out)
+    check_middles(out, stream, w, middle, eps, "norm")
+    at = torch.arange(rows - 1, -1, -1, dtype=torch.int32, device="cuda")
+    o.rmsnorm(x, w.cuda(), eps, out, at)
+    check_middles(out, stream.flip(0), w, middle, eps, "gathered")
+
+
+@GPU
+@pytest.mark.parametrize("res", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("rows,h", NORMS)
+def test_fused_norms_round_the_sum_as_it_was_before_it_was_rounded(rows, h, post, res):
+    """What is added lies below half a unit of the stream's last place (2^-26 of 1): the stream stays as it is, and its norm, in 64 bits, does not.
+    Signs alternate, so that the sum of stream times addend stays far below the sum of squares."""
+    o = ops()
+    stream, w, middle = near_middles(rows, h, 7, seed=h + 1)
+    add = torch.where(torch.arange(h) % 2 == 0, 1.0, -1.0).expand(rows, h) * 2.0 ** -26
+    if post:                                               # a norm of +-1/8 is +-1 exactly
+        r, w_post = (add * 2.0 ** 23).to(res), torch.full((h,), 2.0 ** -26)
+    else:
+        r, w_post = add.to(res), None
+    x, out = stream.cuda(), o.MxRows.empty(rows, h)
+    o.add_rmsnorm(x, r.cuda().contiguous(), w_post.cuda() if post else None, 0.0, w.cuda(), 0.0, out)
+    assert torch.equal(x.cpu(), stream)
+    check_middles(out, stream.double() + add.double(), w, middle, 0.0, "sum")
