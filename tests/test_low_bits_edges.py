@@ -170,3 +170,14 @@ def test_fused_norms_round_the_sum_as_it_was_before_it_was_rounded(rows, h, post
     o.add_rmsnorm(x, r.cuda().contiguous(), w_post.cuda() if post else None, 0.0, w.cuda(), 0.0, out)
     assert torch.equal(x.cpu(), stream)
     check_middles(out, stream.double() + add.double(), w, middle, 0.0, "sum")
+
+
+@GPU
+@pytest.mark.parametrize("rows,h", [(800, 1024), (800, 1280), (1000, 512), (800, 1001)])
+def test_norms_of_many_rows_add_up_in_64_bits(rows, h):
+    """Squares up to 255^2: a warp's sum of 256 is a float, the row's is none.  (At a factor that is a float's rounding off, a fifth of the codes turn.)"""
+    o = ops()
+    stream, w, middle = near_middles(rows, h, 255, seed=h)
+    out = o.MxRows.empty(rows, h)
+    o.rmsnorm(stream.cuda(), w.cuda(), 0.0, out)
+    check_middles(out, stream, w, middle, 0.0, f"{rows} x {h}")
