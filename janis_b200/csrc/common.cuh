@@ -329,9 +329,21 @@ __device__ __forceinline__ float gelu_tanh(float v) {
     return 0.5f * v * (1.0f + tanhf(inner));
 }
 
-// The clamped gate: g = min(gate, limit), u = clamp(up, -limit, limit), g sigmoid(alpha g) (u + up_add)
+// The lesser and the greater of two, NaN where either is one (fminf and fmaxf take the other number then)
+__device__ __forceinline__ float least_or_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float most_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The clamped gate: g = min(gate, limit), u = clamp(up, -limit, limit), g sigmoid(alpha g) (u + up_add); a NaN stays one
 __device__ __forceinline__ float clamped_gate(float gate, float up, float limit, float alpha, float up_add) {
-    const float g = fminf(gate, limit), u = fminf(fmaxf(up, -limit), limit);
+    const float g = least_or_nan(gate, limit), u = least_or_nan(most_or_nan(up, -limit), limit);
     return g / (1.0f + expf(-alpha * g)) * (u + up_add);
 }
 

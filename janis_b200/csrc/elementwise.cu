@@ -267,7 +267,7 @@ gated_act8_bf16_kernel(const bf16* __restrict__ gu, bf16* __restrict__ out, size
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if constexpr (ACT == 2) {
-                const float gg = fminf(g[e], limit), uu = fminf(fmaxf(u[e], -limit), limit);
+                const float gg = least_or_nan(g[e], limit), uu = least_or_nan(most_or_nan(u[e], -limit), limit);
                 o[e] = gg * rcp_fast(1.0f + ex2_fast(-alpha * gg * 1.4426950408889634f)) * (uu + up_add);
             } else {
                 o[e] = (ACT == 0 ? gelu_tanh_fast(g[e]) : silu_fast(g[e])) * u[e];

@@ -181,3 +181,64 @@ def test_norms_of_many_rows_add_up_in_64_bits(rows, h):
     out = o.MxRows.empty(rows, h)
     o.rmsnorm(stream.cuda(), w.cuda(), 0.0, out)
     check_middles(out, stream, w, middle, 0.0, f"{rows} x {h}")
+
+
+# ---------------------------------------------------------------------------
+# groups that stand for NaN, behind a gate
+# ---------------------------------------------------------------------------
+
+CLAMP = dict(limit=1.5, alpha=1.702, up_add=1.0)
+
+
+@GPU
+@pytest.mark.parametrize("epi", [1, 3, 4])
+@pytest.mark.parametrize("t", [3, 40, 300])
+def test_groups_that_stand_for_nan_spoil_what_a_gate_makes_of_them(t, epi):
+    o = ops()
+    x, w = operands(t, 160, 384)
+    x.scales.view(-1)[0] = 255               # row 0, group 0
+    w.scales.view(-1)[16 * 5 + 1] = 255      # row 5, group 1: the gate of column 5
+    w.scales.view(-1)[16 * 26 + 1] = 255     # row 26, group 1: the up of column 10
+    three = CLAMP if epi == 4 else {}
+    for dtype in (torch.float32, torch.bfloat16):
+        out = o.linear_mx(x, w, torch.empty(t, 80, dtype=dtype, device="cuda"), epi, **three)
+        bad = torch.zeros(t, 80, dtype=torch.bool, device="cuda")
+        bad[0], bad[:, 5], bad[:, 10] = True, True, True
+        assert torch.equal(torch.isnan(out), bad)
+    rows = o.MxRows.empty(t, 80)
+    o.linear_mx(x, w, rows, epi, **three)
+    nan = scale_rows(rows) == 255
+    assert nan[0, :3].all() and nan[:, 0].all() and not nan[1:, 1:].any() and not nan[:, 3:].any()
+    assert not rows.codes[:, :32].any() and not rows.codes[0].any()
+
+
+@GPU
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols", [72, 264])
+def test_the_clamped_gate_keeps_nan(cols, dtype):
+    """Alone, into rows and into values (in groups of 8 and of 4), and behind the product of few bfloat16 rows."""
+    o = ops()
+    gate, up = rnd(4, cols, seed=1) * 2, rnd(4, cols, seed=2) * 2
+    gate[0, 3], up[1, 40], gate[2, 1], up[2, 2] = NAN, NAN, INF, -INF
+    for group in (8, 4):
+        gu = torch.stack([gate.view(4, -1, group), up.view(4, -1, group)], 2).reshape(4, 2 * cols).to(dtype)
+        g, u = (v.reshape(4, cols) for v in gu.double().view(4, cols // group, 2, group).unbind(2))
+        want = R._clamped(g, u, *CLAMP.values())
+        bad = torch.isnan(want)
+        assert bad.sum() == 2
+        got = o.gated_act(gu, torch.empty(4, cols, dtype=dtype, device="cuda"), 2, group, **CLAMP)
+        assert torch.equal(torch.isnan(got), bad)
+        # alpha g is up to 14, and its rounding an absolute error of the exponent; some 8 roundings behind it
+        assert ((got.double() - want)[~bad].abs() <= (2.0 ** -8 if dtype == torch.bfloat16 else 22 * 2.0 ** -23) * want[~bad].abs()).all()
+        if group == 8:
+            rows = o.MxRows.empty(4, cols)
+            o.gated_act(gu, rows, 2, **CLAMP)
+            nan = scale_rows(rows) == 255
+            assert nan[0, 0] and nan[1, 1] and nan.sum() == 2
+    if dtype == torch.bfloat16:
+        w = torch.zeros(16, 64, dtype=dtype, device="cuda")
+        w[:8, 0], w[8:, 1] = 1.0, 1.0
+        x = torch.ones(3, 64, dtype=dtype, device="cuda")
+        x[0, 2] = NAN                        # (times zero: every sum of the row)
+        out = o.gemv_bf16(x, w, torch.empty(3, 8, dtype=dtype, device="cuda"), o.EPI_GATED_CLAMP, cap=1.5, alpha=1.702, up_add=1.0)
+        assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
