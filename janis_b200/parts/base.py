@@ -162,10 +162,13 @@ class Workspace:
     def mx_rows(self, name: str, n_rows: int, width: int, cls):
         """The same for rows in 8 bits (`cls`: the kernels' `MxRows`).  Whoever writes such rows writes their padding too."""
         kp = -(-width // 128) * 128
+        last = self._rows.get(name)
+        if last is None or last.rows != n_rows or last.width != width:
+            last = None                           # (nor may it hold the memory that `buf` is about to give up)
+            self._rows.pop(name, None)
         codes = self.buf(name + ".codes", (n_rows, kp), torch.uint8)
         scales = self.buf(name + ".scales", (-(-n_rows // 128), kp // 128, 512), torch.uint8)
-        last = self._rows.get(name)
-        if last is None or last.codes is not codes or last.scales is not scales or last.width != width:
+        if last is None or last.codes is not codes or last.scales is not scales:
             last = self._rows[name] = cls(codes, scales, n_rows, width)
         return last
 

@@ -242,3 +242,46 @@ def test_the_clamped_gate_keeps_nan(cols, dtype):
         x[0, 2] = NAN                        # (times zero: every sum of the row)
         out = o.gemv_bf16(x, w, torch.empty(3, 8, dtype=dtype, device="cuda"), o.EPI_GATED_CLAMP, cap=1.5, alpha=1.702, up_add=1.0)
         assert torch.isnan(out[0]).all() and torch.isfinite(out[1:]).all()
+
+
+# ---------------------------------------------------------------------------
+# the workspace
+# ---------------------------------------------------------------------------
+
+def test_room_for_rows_goes_before_more_of_it_comes(monkeypatch):
+    from janis_b200.parts.base import Workspace
+    ws = Workspace("cpu")
+    held = [weakref.ref(t.untyped_storage()) for m in [ws.mx_rows("y", 130, 200, R.MxRows)] for t in (m.codes, m.scales)]
+    alive = []
+
+    def zeros(*a, **kw):
+        gc.collect()
+        alive.append([r() is not None for r in held])
+        return made(*a, **kw)
+
+    made = torch.zeros
+    monkeypatch.setattr(torch, "zeros", zeros)
+    m = ws.mx_rows("y", 300, 200, R.MxRows)
+    assert alive[0][0] is False, "the old codes were still there when the new ones came"
+    assert alive[-1] == [False, False]
+    assert m.shape == (300, 200) and ws.mx_rows("y", 300, 200, R.MxRows) is m
+    monkeypatch.undo()
+    fewer = ws.mx_rows("y", 7, 200, R.MxRows)
+    assert fewer.shape == (7, 200) and fewer.codes.data_ptr() == m.codes.data_ptr()
+    narrow = ws.mx_rows("y", 7, 150, R.MxRows)              # of the same padded width
+    assert narrow.shape == (7, 150) and narrow.codes.data_ptr() == m.codes.data_ptr()
+
+
+def test_room_that_a_graph_has_recorded_stays():
+    from janis_b200.parts.base import Workspace
+    ws = Workspace("cpu")
+    small = ws.mx_rows("y", 3, 128, R.MxRows)
+    ws.begin_capture()
+    assert ws.mx_rows("y", 3, 128, R.MxRows) is small
+    with pytest.raises(RuntimeError):
+        ws.mx_rows("y", 300, 128, R.MxRows)
+    ws.end_capture()
+    at = small.codes.data_ptr()
+    del small
+    big = ws.mx_rows("y", 300, 128, R.MxRows)
+    assert big.shape == (300, 128) and big.codes.data_ptr() != at and any(t.data_ptr() == at for t in ws._retired)
