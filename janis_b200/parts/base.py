@@ -174,10 +174,14 @@ class Workspace:
 
     def fill(self, value) -> None:
         """Every buffer filled with `value` (tests poison the workspace with NaN between steps: a step must write
-        what it reads)."""
+        what it reads).  8-bit rows take values of that size, or codes and scales that stand for NaN."""
         for t in self._bufs.values():
             if t.is_floating_point():
                 t.fill_(value)
+        code = int(torch.tensor(float(value)).to(torch.float8_e4m3fn).view(torch.uint8))
+        for name in self._rows:
+            self._bufs[name + ".codes"].fill_(code)
+            self._bufs[name + ".scales"].fill_(255 if value != value else 127)
 
     def begin_capture(self) -> None:
         self.frozen = True

@@ -285,3 +285,40 @@ def test_room_that_a_graph_has_recorded_stays():
     del small
     big = ws.mx_rows("y", 300, 128, R.MxRows)
     assert big.shape == (300, 128) and big.codes.data_ptr() != at and any(t.data_ptr() == at for t in ws._retired)
+
+
+def test_poison_reaches_rows_in_8_bits():
+    from janis_b200.parts.base import Workspace
+    ws = Workspace("cpu")
+    m, plain = ws.mx_rows("y", 3, 128, R.MxRows), ws.buf("bytes", (8,), torch.uint8)
+    ws.fill(NAN)
+    assert (m.codes == 0x7F).all() and (m.scales == 255).all() and not plain.any()
+    ws.fill(0.0)
+    assert not m.codes.any() and (m.scales == 127).all()
+
+
+@GPU
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_steps_write_every_row_in_8_bits_that_they_read(dtype, model_dirs):
+    """Graphs on, batches that fill their padded shape and such that do not, the workspace poisoned before every step: the logits
+    are those of the same engine without the poison, bit for bit."""
+    from janis_b200 import StepEntry
+    got = []
+    for poisoned in (False, True):
+        eng = mx_engine(model_dirs["C_hot"], dtype, "cuda", max_tokens=2048)
+        logits = []
+        for b, lens in enumerate([(30, 75, 12), (41, 50, 33), (64, 64), (1, 100, 20), (3, 2, 1), (120,)]):
+            reqs = [random_tokens(TINY["C"]["vocab_size"], n + 3, 500 + 10 * b + i) for i, n in enumerate(lens)]
+            slots = [eng.alloc_slot() for _ in reqs]
+            for t in range(-1, 3):
+                if poisoned:
+                    eng.stepper.ws.fill(NAN)
+                batch = [StepEntry(s, r[:n], [n - 1]) if t < 0 else StepEntry(s, [r[n + t]], [0]) for s, r, n in zip(slots, reqs, lens)]
+                logits.append(eng.step(batch).clone())
+            for s in slots:
+                eng.free_slot(s)
+        assert eng.stepper._prompt_graphs
+        eng.close()
+        got.append(logits)
+    for a, b in zip(*got):
+        assert torch.isfinite(b).all() and torch.equal(a, b)
