@@ -144,6 +144,8 @@ def norm_to_rows(h, res, w_post, eps_post, w_next, eps_next, out: MxRows, n_part
         return out
     H = shape[1]
     R = out.rows if res is None else shape[0]
+    if n_part < 1:
+        raise _ops.KernelError("add_rmsnorm: n_part must be >= 1")
     if w_next is None:
         raise _ops.KernelError("add_rmsnorm: 8-bit rows are the second norm's output, which has no weight here")
     t = _ops._t
@@ -166,8 +168,10 @@ def gated_to_rows(gu, out: MxRows, act: int, group: int, limit: float, alpha: fl
     R, I2 = gu.shape
     if group != _ops.GATE_GROUP:
         raise _ops.KernelError(f"gated_act: 8-bit rows come from gates and ups in groups of {_ops.GATE_GROUP}, found {group}")
+    if act not in (_ops.ACT_GELU_TANH, _ops.ACT_SILU, _ops.ACT_CLAMPED):
+        raise _ops.KernelError(f"gated_act: unknown activation {act}")
     lib = _ops.low_bits()
-    _ops._check(lib, lib.janis_mx_rows(_ops._t(gu, "gu", _ops._FLOATS), _ops._DT[gu.dtype], int(act), float(limit), float(alpha), float(up_add),
+    _ops._check(lib, lib.janis_mx_rows(_ops._t(gu, "gu", _ops._FLOATS, (R, I2 // 2 * 2)), _ops._DT[gu.dtype], int(act), float(limit), float(alpha), float(up_add),
                                        *_rows(out, "out", R, I2 // 2), R, I2 // 2, _ops._stream()))
     return out
 

@@ -344,6 +344,8 @@ def add_rmsnorm(h, res, w_post, eps_post, w_next=None, eps_next=0.0, out=None, n
     out = norm(h; w_next) when w_next is given.
     `res` is [R, H], or [n_part, R, H] partial results that are added first.  `out` may be `MxRows`."""
     if type(out) is MxRows:
+        if res is None:
+            raise KernelError("res: expected a CUDA tensor")
         return mx.norm_to_rows(h, res, w_post, eps_post, w_next, eps_next, out, n_part)
     R, H = h.shape
     if n_part == 1:

@@ -322,3 +322,21 @@ def test_steps_write_every_row_in_8_bits_that_they_read(dtype, model_dirs):
         got.append(logits)
     for a, b in zip(*got):
         assert torch.isfinite(b).all() and torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------
+# refusals
+# ---------------------------------------------------------------------------
+
+@GPU
+def test_what_the_plain_forms_refuse_is_refused_with_rows_behind_it():
+    o = ops()
+    y, plain, w = o.MxRows.empty(4, 64), torch.empty(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    for out in (y, plain):
+        for bad in (lambda: o.gated_act(rnd(4, 128), out, -1), lambda: o.gated_act(rnd(4, 128), out, 3), lambda: o.gated_act(rnd(4, 129), out),
+                    lambda: o.add_rmsnorm(rnd(4, 64), None, w, 0.0, w, 0.0, out),
+                    lambda: o.add_rmsnorm(rnd(4, 64), torch.empty(0, 4, 64, device="cuda"), w, 0.0, w, 0.0, out, n_part=0),
+                    lambda: o.add_rmsnorm(rnd(4, 64), rnd(4, 64), w[::2], 0.0, w, 0.0, out)):
+            with pytest.raises((o.KernelError, AttributeError)):
+                bad()
+    torch.cuda.synchronize()
