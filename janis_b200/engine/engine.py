@@ -239,7 +239,8 @@ def open(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, max_batch: in
     rt = _runtime(dtype, device, weights)
     if rt.weights:
         check_low_bits(model)
-    store = WeightStore(load_tensors(model_dir, model.tensor_specs(), rt.device, model.ignorable_tensors))
+    store = WeightStore(load_tensors(model_dir, model.tensor_specs(), rt.device, model.ignorable_tensors,
+                                     keep_half=rt.weight_dtype is None))
     model.load(store, rt)         # parts that fuse tensors give the stored ones up as they go
     del store
     return Engine(model, rt, max_tokens, max_batch, max_context, max_step_tokens, use_graphs)

@@ -81,7 +81,9 @@ class Runtime:
 
     def weight(self, w: torch.Tensor):
         """A matrix of a layer's product as the product takes it: as it is, or in 4 bits."""
-        return self.ops.mx_weight(w.contiguous()) if self.weights == "mx4" else w.contiguous()
+        if self.weights == "mx4":
+            return self.ops.mx_weight((w.float() if w.dtype == torch.float16 else w).contiguous())
+        return w.contiguous()
 
     def rows(self, ws: "Workspace", name: str, n_rows: int, width: int):
         """Room for the rows a layer's product reads: in the compute dtype, or in 8 bits."""

@@ -4,8 +4,9 @@ A model states which tensors it expects (`TensorSpec` by checkpoint name); the
 loader compares that with what the folder holds and raises ONE error that lists
 every missing tensor, every unexpected tensor and every wrong shape.  What is
 loaded is kept as stored where it can be: BF16 stays bfloat16, F16 becomes
-bfloat16, anything stored in 32-bit floating point stays float32, integer
-tables become int32.  The parts widen to float32 themselves when the engine
+bfloat16 (or stays, for whoever goes on to fewer bits from there), anything
+stored in 32-bit floating point stays float32, integer tables become int32.
+The parts widen to float32 themselves when the engine
 runs its 32-bit path.
 
 The reference loads tensor by tensor through `File.Get(name)` and fails on the
@@ -77,18 +78,20 @@ def check_tensors(expected: Mapping[str, TensorSpec], files: ModelFiles,
     raise WeightsError("\n".join(lines))
 
 
-def stored_to_kept(t: torch.Tensor, integer: bool) -> torch.Tensor:
+def stored_to_kept(t: torch.Tensor, integer: bool, keep_half: bool = False) -> torch.Tensor:
     """The dtype a tensor is kept in after loading (see the module text)."""
     if integer:
         return t.to(torch.int32)
     if t.dtype in (torch.float32, torch.float64):
         return t.to(torch.float32)
+    if keep_half and t.dtype == torch.float16:
+        return t
     return t.to(torch.bfloat16)
 
 
 def load_tensors(model_dir: str, expected: Mapping[str, TensorSpec], device,
-                 ignorable: Iterable[str] = ()) -> dict[str, torch.Tensor]:
-    """Check the folder against `expected`, then bring every expected tensor to `device`."""
+                 ignorable: Iterable[str] = (), keep_half: bool = False) -> dict[str, torch.Tensor]:
+    """Check the folder against `expected`, then bring every expected tensor to `device` (`keep_half`: F16 as it is)."""
     try:
         files = open_model(model_dir)
     except SafetensorsError as e:
@@ -97,7 +100,7 @@ def load_tensors(model_dir: str, expected: Mapping[str, TensorSpec], device,
         check_tensors(expected, files, ignorable)
         out = {}
         for name, spec in expected.items():
-            out[name] = stored_to_kept(files.read(name), spec.integer).to(device)
+            out[name] = stored_to_kept(files.read(name), spec.integer, keep_half).to(device)
         return out
     finally:
         files.close()

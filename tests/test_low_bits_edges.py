@@ -340,3 +340,52 @@ def test_what_the_plain_forms_refuse_is_refused_with_rows_behind_it():
             with pytest.raises((o.KernelError, AttributeError)):
                 bad()
     torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------------------
+# weights as they are stored
+# ---------------------------------------------------------------------------
+
+def half_folder(folder, tmp_path):
+    """The folder's model with its tensors as F16, values that bfloat16 would round among them."""
+    import json
+    import os
+    from janis_b200.weights.loader import write_model_folder
+    from tests.plain import gemma2_plain as P
+    cfg, w = P.load_folder(folder)
+    half = {}
+    for i, (name, t) in enumerate(sorted(w.items())):
+        half[name] = (t.float() * (1 + 0.01 * torch.rand(t.shape, generator=torch.Generator().manual_seed(i)))).half()
+    with open(os.path.join(folder, "config.json"), encoding="utf-8") as f:
+        write_model_folder(str(tmp_path / "half"), json.load(f), half)
+    return str(tmp_path / "half"), half
+
+
+def check_half(model, half):
+    for i, blk in enumerate(model.blocks):
+        p = f"model.layers.{i}."
+        down, o = (R.quantised(half[p + n].double(), *E2M1)[0] for n in ("mlp.down_proj.weight", "self_attn.o_proj.weight"))
+        qkv = torch.cat([R.quantised(half[p + f"self_attn.{n}_proj.weight"].double(), *E2M1)[0] for n in "qkv"])
+        for got, want in ((blk.feed_forward.w_down, down), (blk.mixer.w_o, o), (blk.mixer.w_qkv, qkv)):
+            assert torch.equal(got.values().double().cpu()[:, :want.shape[1]], want)
+
+
+@pytest.mark.parametrize("on", ["refs", pytest.param("cuda", marks=GPU)])
+def test_half_precision_files_are_converted_from_what_they_hold(on, model_dirs, tmp_path):
+    folder, half = half_folder(model_dirs["A"], tmp_path)
+    w = half["model.layers.0.mlp.down_proj.weight"]
+    assert not torch.equal(R.quantised(w.double(), *E2M1)[0], R.quantised(w.bfloat16().double(), *E2M1)[0])
+    if on == "cuda":
+        eng = mx_engine(folder, "float32", on, max_tokens=256)
+        check_half(eng.model, half)
+        eng.close()
+        return
+    from janis_b200.config.base import read_config_json
+    from janis_b200.engine.engine import build_model
+    from janis_b200.parts.base import Runtime, WeightStore
+    from janis_b200.weights.loader import load_tensors
+    _, _, model = build_model(read_config_json(folder))
+    model.load(WeightStore(load_tensors(folder, model.tensor_specs(), "cpu", keep_half=True)), Runtime(torch.bfloat16, "cpu", R, "mx4"))
+    check_half(model, half)
+    # where nothing goes on to 4 bits they become bfloat16 as before
+    assert load_tensors(folder, model.tensor_specs(), "cpu")["model.embed_tokens.weight"].dtype == torch.bfloat16
