@@ -17,7 +17,7 @@ import torch
 from ..cache.cache import ModelCache
 from ..config.base import ConfigError, read_config_json
 from ..kernels import ops as cuda_ops
-from ..parts.base import Runtime, WeightStore
+from ..parts.base import Norm, Runtime, WeightStore
 from ..registry import resolve
 from ..sampling.sampler import Sampler, SamplingParams
 from ..weights.loader import load_tensors, random_tensors, write_model_folder
@@ -210,11 +210,12 @@ def _runtime(dtype, device, weights=None) -> Runtime:
 
 
 def check_low_bits(model) -> None:
-    """Refuses a model some of whose layers cannot keep their matrices in 4 bits."""
+    """Refuses a model some of whose layers cannot keep their matrices in 4 bits, or whose norms in front of them leave no 8-bit rows."""
     for i, blk in enumerate(model.blocks):
-        for part in (blk, blk.mixer, getattr(blk, "feed_forward", None)):
+        for part in (blk, *(getattr(blk, name, None) for name in ("mixer", "feed_forward", "first_norm", "pre_ff_norm"))):
             if part is not None and not part.low_bits:
-                raise ValueError(f"weights='mx4': {type(part).__name__} (layer {i}) takes its matrices in the compute dtype only")
+                what = "leaves rows" if isinstance(part, Norm) else "takes its matrices"
+                raise ValueError(f"weights='mx4': {type(part).__name__} (layer {i}) {what} in the compute dtype only")
 
 
 def build_model(raw_config: dict, where: str = "config.json"):

@@ -229,7 +229,8 @@ class Part:
     # leaves it True meets padding in recorded steps, decode and prompt steps alike: sequences whose slot is
     # negative (and the tokens that name them) must be stored nowhere and must change no other row.
     graph_safe = True
-    # whether a block, mixer or feed-forward keeps its matrices through `rt.weight` and takes its rows as `rt.rows` gives them
+    # whether a block, mixer or feed-forward keeps its matrices through `rt.weight` and takes its rows as `rt.rows` gives them;
+    # whether a norm in front of one leaves such rows
     low_bits = False
 
     def tensor_specs(self) -> dict[str, TensorSpec]:

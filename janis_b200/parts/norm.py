@@ -30,6 +30,8 @@ from .base import Norm, Part, Runtime, StepContext
 
 
 class RMSNorm(Norm):
+    low_bits = True
+
     def __init__(self, width: int, eps: float, weight_name: str, offset: float = 0.0, init_std: float = 0.1,
                  init_mean: float = 0.0):
         self.width = width

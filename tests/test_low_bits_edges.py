@@ -389,3 +389,16 @@ def test_half_precision_files_are_converted_from_what_they_hold(on, model_dirs, 
     check_half(model, half)
     # where nothing goes on to 4 bits they become bfloat16 as before
     assert load_tensors(folder, model.tensor_specs(), "cpu")["model.embed_tokens.weight"].dtype == torch.bfloat16
+
+
+def test_a_norm_that_leaves_no_8_bit_rows_is_refused():
+    import janis_b200
+    from janis_b200.engine.engine import check_low_bits
+    from janis_b200.parts import registry as parts
+    from tests.conftest import TINY_A
+    for where in ("first_norm", "pre_ff_norm"):
+        _, _, model = janis_b200.build_model(TINY_A)
+        check_low_bits(model)
+        setattr(model.blocks[1], where, parts.make("norm", "layer_norm", width=64, eps=1e-6, weight_name="n"))
+        with pytest.raises(ValueError, match="LayerNorm.*layer 1"):
+            check_low_bits(model)
