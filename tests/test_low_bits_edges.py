@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes
 import gc
-import math
 import weakref
 
 import pytest
@@ -16,7 +15,7 @@ import torch
 from tests import kernel_refs as R
 from tests.conftest import F32_MODEL_TOL, TINY, random_tokens
 from tests.helpers import run_requests
-from tests.test_low_bits import E2M1, E4M3, code_values, far, mx_engine, operands, ops, plain_mx_logits, powers, rnd, scale_rows, stands_for
+from tests.test_low_bits import E2M1, E4M3, code_values, far, mx_engine, operands, ops, plain_mx_logits, rnd, scale_rows
 
 GPU = pytest.mark.gpu
 INF, NAN = float("inf"), float("nan")
@@ -402,3 +401,41 @@ def test_a_norm_that_leaves_no_8_bit_rows_is_refused():
         setattr(model.blocks[1], where, parts.make("norm", "layer_norm", width=64, eps=1e-6, weight_name="n"))
         with pytest.raises(ValueError, match="LayerNorm.*layer 1"):
             check_low_bits(model)
+
+
+# ---------------------------------------------------------------------------
+# waits that were given up, whole models
+# ---------------------------------------------------------------------------
+
+@GPU
+def test_the_engine_says_when_a_wait_of_this_library_was_given_up(monkeypatch, model_dirs):
+    """The count of given-up waits comes from a stand-in for the entry point (no kernel is made to wait in vain)."""
+    import janis_b200
+    from janis_b200.kernels import ops as o
+    eng = janis_b200.open(model_dirs["A"], dtype="bfloat16", max_tokens=512, weights="mx4")
+    prompts = [random_tokens(TINY["A"]["vocab_size"], n, n) for n in (9, 30)]
+    first = eng.generate(prompts, max_tokens=5, stop=())
+    real, count = o._low_bits, [0]
+
+    class Library:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def janis_mx_timeouts_async(self, host, stream):
+            ctypes.c_int.from_address(host).value = count[0]
+            return 0
+
+    monkeypatch.setattr(o, "_low_bits", Library())
+    assert eng.generate(prompts, max_tokens=5, stop=()) == first
+    count[0] = 2
+    with pytest.raises(o.KernelError, match="2 in low_bits"):
+        eng.generate(prompts, max_tokens=5, stop=())
+    assert eng.cache.live_slots() == []
+    eng.cache.audit()
+    assert eng.generate(prompts, max_tokens=5, stop=()) == first
+    count[0] = 3
+    with pytest.raises(o.KernelError, match="1 in low_bits"):
+        eng.check_health()
+    eng.check_health()
+    monkeypatch.undo()
+    eng.close()
