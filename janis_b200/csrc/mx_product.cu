@@ -444,15 +444,22 @@ __device__ __forceinline__ void no_columns_from(uint32_t* v, int left) {
     for (int j = 0; j < COUNT; ++j) v[j] = j < left ? v[j] : 0u;
 }
 
+// Holds what is made of `v` behind the arrival that gives tensor memory back: values of an asm volatile stay behind those before it.  Without it the
+// compiler may move the activation in front, and the next tile's products wait for it: 2,048 rows x 18,432 x 2,304 took 82 us then, 75 with it behind.
+template <int COUNT>
+__device__ __forceinline__ void keep_behind(uint32_t (&v)[COUNT]) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) asm volatile("" : "+r"(v[j]));
+}
+
 // The end of a row's run of COLS columns of sums from column n0 on (rows of W), by the thread that holds them; a whole warp calls it.
 template <int COLS, int EPI>
 __device__ __forceinline__ void finish_run(uint32_t (&v)[COLS], const Out& o, int t, int n0, int T, int N, int vec) {
     if constexpr (EPI == EPI_NONE) {
         store_run<COLS>(v, o, t, n0, T, N, vec);
     } else {
-        // (a branch here also keeps the activation behind the arrival that gives tensor memory back: without one the compiler moves it in
-        // front, and 2,048 rows x 18,432 x 2,304 take 82 us instead of 75)
         if (t >= T && (vec != 0 || o.codes != nullptr)) return;
+        keep_behind(v);
         const int cols = N / 2, wide = o.codes != nullptr ? padded(cols) : cols, c = n0 / 2;
 #pragma unroll
         for (int u = 0; u < COLS / 16; ++u)
