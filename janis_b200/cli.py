@@ -22,7 +22,7 @@ import time
 USAGE = """usage: janis generate --model DIR (--ids 1,2,3 | --ids-file FILE) [--temp 0] [--top-p 1] [--max-tokens 512]
                       [--seed 0] [--stop 1,107] [--dtype bfloat16|float32] [--max-cache-tokens N] [--weights mx4]
        janis generate --random CONFIG.json [--weights-seed 0] ...   (random weights instead of a folder)
-       janis replay   --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N   < steps.jsonl
+       janis replay   --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N [--weights mx4]   < steps.jsonl
        janis random   --config CONFIG.json --out DIR [--seed 0]     (write a folder of random weights)
        janis bench    [--steps K] [--warmup W] [--batch 8] [--context 8192] [--layers N]
        janis version"""

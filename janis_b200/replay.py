@@ -87,6 +87,7 @@ def main(argv=None) -> int:
     ap.add_argument("--max-tokens", type=int, required=True,
                     help="most tokens that live requests hold at any time; sizes the cache (with room to spare for partly filled pages)")
     ap.add_argument("--no-graphs", action="store_true", help="launch decode steps kernel by kernel")
+    ap.add_argument("--weights", default=None, choices=["mx4"], help="keep the layers' matrices in 4 bits")
     args = ap.parse_args(argv)
     from .engine import engine as eng_mod
     from .config.base import read_config_json
@@ -96,7 +97,7 @@ def main(argv=None) -> int:
     max_tokens = max(64, args.max_tokens) + 64 * 256
     ctx = max(int(raw.get("max_position_embeddings", 0) or 0), (max_tokens + 63) // 64 * 64)
     engine = eng_mod.open(args.model, dtype=args.dtype, max_tokens=max_tokens, max_context=ctx,
-                          use_graphs=not args.no_graphs)
+                          use_graphs=not args.no_graphs, weights=args.weights)
     try:
         run_trace(engine, iter(sys.stdin.readline, ""), args.out)
     finally:

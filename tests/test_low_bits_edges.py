@@ -457,3 +457,25 @@ def test_most_requests_agree_to_a_floats_precision(model_dirs, plain_models):
         all_of_them += len(reqs)
         eng.close()
     assert close > all_of_them // 2, f"{close} of {all_of_them}"
+
+
+@GPU
+def test_replay_takes_4_bit_weights(model_dirs, tmp_path, monkeypatch):
+    import io
+    import json
+    import sys
+    import numpy as np
+    from janis_b200 import StepEntry
+    from janis_b200.replay import main
+    ids, vocab = random_tokens(TINY["A"]["vocab_size"], 12, 3), TINY["A"]["vocab_size"]
+    steps = [{"step": 0, "entries": [{"id": "a", "tokens": ids[:11], "want": [0, 10]}], "end": []},
+             {"step": 1, "entries": [{"id": "a", "tokens": ids[11:], "want": [0]}], "end": ["a"]}]
+    monkeypatch.setattr(sys, "stdin", io.StringIO("".join(json.dumps(s) + "\n" for s in steps)))
+    assert main(["--model", model_dirs["A"], "--dtype", "float32", "--out", str(tmp_path), "--max-tokens", "64", "--weights", "mx4", "--no-graphs"]) == 0
+    eng = mx_engine(model_dirs["A"], "float32", "cuda", max_tokens=256, use_graphs=False)
+    slot = eng.alloc_slot()
+    for i, entry in enumerate((StepEntry(slot, ids[:11], [0, 10]), StepEntry(slot, ids[11:], [0]))):
+        want = eng.step([entry]).cpu()
+        got = torch.from_numpy(np.fromfile(tmp_path / f"{i}.f32", dtype="<f4")).view(-1, vocab)
+        assert torch.equal(got, want)
+    eng.close()
