@@ -628,6 +628,7 @@ constexpr int PAIR_SMEM = PAIR_STAGES * (PAIR_STAGE + PAIR_SCALES) + 1024;
 // 256 rows of x by 256 of W: each SM holds half of both, so that it fetches and reads two thirds of what a tile of 128 x 256 wants for the same
 // products, and its sums are 128 rows of 256 columns.  At prompts' sizes the products are bound by the power limit (1.1 to 1.5 GHz), so that what
 // a tile does not fetch counts: 2,048 rows x 4,608 x 36,864 254 us, against 274 with tiles of 128 x 256 of one SM and 333 of 128 x 128.
+// (Without a gate the 128 columns of a thread and what it stores them by spill 84 bytes.)
 // Tensor memory holds one tile's sums, and the products wait some 2 us while they are taken out.  Tiles of 256 x 192, of which it holds two, close
 // that gap and are no faster: 2,048 x 18,432 x 2,304 gated 74.5 us against 73.4, 2,048 x 4,608 x 36,864 281 against 255.
 template <int EPI>

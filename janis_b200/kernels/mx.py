@@ -183,7 +183,7 @@ def mx_set_few(split: int = 0, stages: int = 0) -> None:
 
 def mx_set_kernel(kernel: int = 0) -> None:
     """Fixes the kernel of products: 0 chosen by their sizes, 1 few rows, 2 and 3 many rows by pairs of CTAs and by one, 4 many rows whose K
-    is shared by the CTAs of `mx_set_few`.  For tests and tuning."""
+    is shared by the CTAs of `mx_set_few`, 5, 6 and 7 the same by 2, 4 and 8 of them.  For tests and tuning."""
     _ops.low_bits().janis_mx_set_kernel(int(kernel))
 
 
