@@ -135,7 +135,8 @@ __device__ __forceinline__ void store_eight_of_group(const float* v, uint8_t* co
 // thread; of 2,303 98 (loads and stores of single values).  Rows above 4,096 leave room for one block of 8 values a thread on an SM (64
 // registers, 513 threads or more): with 16 there are two, 2,048 rows of 4,607 62.9 us against 82.1, 256 10.0 against 12.5; a single row, which
 // has the SM to itself, 6.6 against 5.3; 16 spill 72 bytes, 40 with a float residual.  All of these are 2.6 to 4 times what the bytes take (13.8 us for
-// 8,192 of 1,001, 31.8 of 2,303; 15.9 for 2,048 of 4,607), with neither memory nor issue slots at their limit.  Rows brought in 16-byte pieces through shared memory: 41.6 us (of 1,001), 105 (of 2,303), 62.8 (of 4,607).
+// 8,192 of 1,001, 31.8 of 2,303; 15.9 for 2,048 of 4,607), with neither memory nor issue slots at their limit.  Rows brought in 16-byte pieces
+// through shared memory: 41.6 us (of 1,001), 105 (of 2,303), 62.8 (of 4,607).
 template <typename TR, int VPT>
 __global__ void __launch_bounds__(640)
 norm_rows_odd_kernel(float* __restrict__ h, const TR* __restrict__ res, const float* __restrict__ w_post, float eps_post,
@@ -225,10 +226,11 @@ template <> struct Eight<float> {
 // many rows an SM has on its way: the residual stays as it is stored, the norms' weights are read where they are used, and a thread takes two
 // pieces.  8,192 rows of 2,304 over the same inputs, in us: one piece a thread 43.2, two 37.9, five 40.3, nine (a warp a row) 59.8; 31.9 at the copy's
 // bandwidth.  With the warps' sums in 64 bits and values near a middle formed again 40.7, over inputs that L2 does not hold 43 to 44, for half as many codes
-// that differ from those of 64 bits (69 of 75 million; plain float arithmetic 144).  Held weights and eight floats of the residual a thread: 60.0; rows that the copy engine brings into a
-// ring: 66.7.  At few rows, bound by latency, one piece: one row 2.5 us, with two 2.8.
+// that differ from those of 64 bits (69 of 75 million; plain float arithmetic 144).  Held weights and eight floats of the residual a thread: 60.0;
+// rows that the copy engine brings into a ring: 66.7.  At few rows, bound by latency, one piece: one row 2.5 us, with two 2.8.
+// At most 48 registers, since what is rare takes more otherwise; two pieces spill 28 bytes, 44 with a float residual.
 template <typename TR, int VPT>
-__global__ void __launch_bounds__(640, VPT == 3 ? 1 : 2)      // (48 registers at most: what is rare takes more otherwise; two pieces spill 28 bytes, 44 with a float residual)
+__global__ void __launch_bounds__(640, VPT == 3 ? 1 : 2)
 norm_rows_vec_kernel(float* __restrict__ h, const TR* __restrict__ res, const float* __restrict__ w_post, float eps_post,
                       const float* __restrict__ w_next, float eps_next, const int* __restrict__ rows, uint8_t* __restrict__ codes,
                       uint8_t* __restrict__ scales, int H, double share) {
